@@ -450,6 +450,96 @@ typedef struct nd_rmsnorm_args {
 
 ND_API int nd_op_rmsnorm(const nd_rmsnorm_args* args, void* stream);
 
+/* ------------------------------------------------------------ residual norm
+ * The norms around a block's branch (attention, MLP) with its gate and
+ * residual, in one pass over the rows:
+ *   x' = residual_scale * x + gate[v] * post(branch)
+ *   y  = pre(x') * (1 + scale[v]) + shift[v]
+ * post / pre: ND_NORM_*, times (weight + plus_one) where a weight is given
+ * (Layers.RmsNorm, src/NaiveDiffusion/Graph/Layers.cs:209-221; LayerNorm and
+ * modulation as Transformer.Modulate, Graph/Transformer.cs:72-80). Row r
+ * reads vector set v = min(r / rows_per_vec, vecs - 1): one set per batch
+ * item, or a dual stream's two. Everything is computed in fp32; y is the next
+ * linear layer's input, in int8 with one scale per row for nd_op_linear_w8a8
+ * (as nd_op_quantize_rows forms it, from the fp32 y). width <= 16384, any
+ * row stride >= width; widths, strides and pointers that are multiples of
+ * four elements run on vector accesses. */
+#define ND_NORM_NONE 0
+#define ND_NORM_RMS 1    /* x * rsqrt(mean(x^2) + eps) */
+#define ND_NORM_LAYER 2  /* (x - mean) * rsqrt(var + eps) */
+
+typedef struct nd_residual_norm_args {
+  int64_t rows, width;
+  const float* x; int64_t ldx;
+  float* x_out; int64_t ldxo;  /* x'; may be x itself (with its stride), else disjoint from x;
+                                  NULL: x' is not stored */
+  const void* branch; int64_t ldb;  /* NULL: x' = residual_scale * x */
+  int branch_dtype;            /* ND_F32, ND_F16 or ND_BF16 */
+  int post_norm;               /* ND_NORM_* over the branch */
+  const float* post_weight;    /* [width] or NULL (factor 1) */
+  const float* gate;           /* [vecs][vec_stride] or NULL (1) */
+  float residual_scale;
+  int pre_norm;                /* ND_NORM_* over x' */
+  const float* pre_weight;     /* [width] or NULL (factor 1) */
+  const float* scale;          /* [vecs][vec_stride] or NULL (0) */
+  const float* shift;          /* [vecs][vec_stride] or NULL (0) */
+  int64_t vecs, vec_stride, rows_per_vec;
+  int plus_one;                /* both weights are stored minus one */
+  float eps;
+  void* y; int64_t ldy;        /* NULL: x' only */
+  int out_dtype;               /* ND_F32, ND_F16, ND_BF16 or ND_I8 */
+  float* y_scale;              /* [rows], ND_I8 only */
+} nd_residual_norm_args;
+
+ND_API int nd_op_residual_norm(const nd_residual_norm_args* args, void* stream);
+
+/* ------------------------------------------------------------ int8 rows
+ * Activations [rows, cols] (f32 / f16 / bf16, row stride ldx) as int8 with one
+ * scale per row (token), the input of nd_op_linear_w8a8:
+ *   scale[r] = max |x[r]| / 127,  q[r, c] = rint(x[r, c] * 127 / max |x[r]|)
+ * with the quotient rounded as if exact, half to even. A row of zeros has
+ * scale 0; a row that holds an infinity or a NaN has scale NaN and q 0.
+ * Columns of q at and past cols are not written. The weights' counterpart is
+ * nd_op_quantize (quant_group 0: one scale per output channel). */
+ND_API int nd_op_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int8_t* q,
+                               int64_t ldq, float* scale, void* stream);
+
+/* ------------------------------------------------------------ int8 x int8 GEMM
+ * y[r, c] = epilogue(x_scale[r] * w_scale[c] * sum_k x[r, k] * weight[c, k] + bias[c])
+ * with int8 x (one scale per row: nd_op_quantize_rows, or nd_op_residual_norm
+ * with an int8 y) and int8 weight (one scale per output channel:
+ * nd_op_quantize with quant_group 0 and fp32 scales). The sum is exact in 32-bit
+ * integers (in_features < 131072). nd_op_linear's weight-only int8 widens the
+ * weights and multiplies in 16 bits; this is the 8-bit product itself.
+ * Row groups (group_split, shared_weights), the epilogues and their operands
+ * are nd_linear_args'; QK_NORM_ROPE is not offered (nd_op_head_norm_rope runs
+ * after a STORE). */
+typedef struct nd_linear_w8a8_args {
+  int dtype;            /* ND_BF16 or ND_F16: y and addend */
+  int epilogue;         /* ND_EPI_* except QK_NORM_ROPE */
+  int64_t rows, in_features, out_features;
+  const int8_t* x;      /* [rows, ldx], ldx % 16 == 0, 16-byte aligned */
+  int64_t ldx;
+  const float* x_scale; /* [rows] */
+  const int8_t* weight; /* [groups * out_features, ldw] (SWIGLU, GEGLU: [2 * out_features, ldw]),
+                           ldw % 16 == 0, 16-byte aligned */
+  int64_t ldw;          /* 0: in_features */
+  const float* w_scale; /* one per weight row */
+  const float* bias;    /* one per weight row, or with shared_weights [groups][...]; NULL: 0 */
+  int64_t group_split;  /* first row of group 1; >= rows for one group */
+  int shared_weights;   /* 1: one weight matrix, bias / gate chosen per row */
+  void* y;              /* [rows, ldy], 16-byte aligned, ldy % 8 == 0 */
+  int64_t ldy;
+  float* residual;      /* [rows, ldr] fp32 (RESIDUAL_*, STORE_F32), 16-byte aligned, ldr % 4 == 0 */
+  int64_t ldr;
+  const float* gate;    /* [groups][gate_stride] (RESIDUAL_GATE) */
+  int64_t gate_stride;  /* 0: out_features */
+  const void* addend;   /* ADD_STORE: [rows, ld_add], dtype like y */
+  int64_t ld_add;
+} nd_linear_w8a8_args;
+
+ND_API int nd_op_linear_w8a8(const nd_linear_w8a8_args* args, void* stream);
+
 /* ------------------------------------------------------------ GEMV
  * y[b, n] = act(sum_k W[n, k] * pre(x[b, k]) + bias[n]), W bf16/f16 [n, k],
  * x and y fp32, batch 1..4. pre_silu applies SiLU to x first; act 0 none,

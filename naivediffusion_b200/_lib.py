@@ -37,6 +37,8 @@ ND_EPI_ADD_STORE = 8
 ND_EPI_SWIGLU = 9
 ND_EPI_GEGLU = 10
 
+ND_NORM_NONE, ND_NORM_RMS, ND_NORM_LAYER = 0, 1, 2
+
 
 class NdError(RuntimeError):
     """A nonzero status from the library, with nd_last_error()'s message."""
@@ -106,6 +108,32 @@ class RmsNormArgs(C.Structure):
     ]
 
 
+class ResidualNormArgs(C.Structure):
+    _fields_ = [
+        ("rows", C.c_int64), ("width", C.c_int64),
+        ("x", C.c_void_p), ("ldx", C.c_int64), ("x_out", C.c_void_p), ("ldxo", C.c_int64),
+        ("branch", C.c_void_p), ("ldb", C.c_int64), ("branch_dtype", C.c_int),
+        ("post_norm", C.c_int), ("post_weight", C.c_void_p), ("gate", C.c_void_p),
+        ("residual_scale", C.c_float), ("pre_norm", C.c_int), ("pre_weight", C.c_void_p),
+        ("scale", C.c_void_p), ("shift", C.c_void_p),
+        ("vecs", C.c_int64), ("vec_stride", C.c_int64), ("rows_per_vec", C.c_int64),
+        ("plus_one", C.c_int), ("eps", C.c_float),
+        ("y", C.c_void_p), ("ldy", C.c_int64), ("out_dtype", C.c_int), ("y_scale", C.c_void_p),
+    ]
+
+
+class LinearW8A8Args(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("epilogue", C.c_int),
+        ("rows", C.c_int64), ("in_features", C.c_int64), ("out_features", C.c_int64),
+        ("x", C.c_void_p), ("ldx", C.c_int64), ("x_scale", C.c_void_p),
+        ("weight", C.c_void_p), ("ldw", C.c_int64), ("w_scale", C.c_void_p), ("bias", C.c_void_p),
+        ("group_split", C.c_int64), ("shared_weights", C.c_int),
+        ("y", C.c_void_p), ("ldy", C.c_int64), ("residual", C.c_void_p), ("ldr", C.c_int64),
+        ("gate", C.c_void_p), ("gate_stride", C.c_int64), ("addend", C.c_void_p), ("ld_add", C.c_int64),
+    ]
+
+
 class GemvArgs(C.Structure):
     _fields_ = [
         ("w", C.c_void_p), ("w_dtype", C.c_int), ("n", C.c_int64), ("k", C.c_int64),
@@ -158,6 +186,10 @@ def lib() -> C.CDLL:
         L.nd_op_rmsnorm.argtypes = [C.POINTER(RmsNormArgs), C.c_void_p]
         L.nd_op_head_norm_rope.argtypes = [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int, C.c_int, C.c_void_p,
                                            C.c_void_p, C.c_void_p, C.c_float, C.c_void_p]
+        L.nd_op_residual_norm.argtypes = [C.POINTER(ResidualNormArgs), C.c_void_p]
+        L.nd_op_quantize_rows.argtypes = [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_void_p,
+                                          C.c_int64, C.c_void_p, C.c_void_p]
+        L.nd_op_linear_w8a8.argtypes = [C.POINTER(LinearW8A8Args), C.c_void_p]
         L.nd_op_gemv.argtypes = [C.POINTER(GemvArgs), C.c_void_p]
         L.nd_op_patchify.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int,
                                      C.c_int, C.c_int, C.c_int64, C.c_void_p]

@@ -60,6 +60,10 @@ int attention_f32(const nd_attention_args& a, cudaStream_t stream);
 int sampler_step(const nd_sampler_args& a, cudaStream_t stream);
 int modulate(const nd_modulate_args& a, cudaStream_t stream);
 int rmsnorm(const nd_rmsnorm_args& a, cudaStream_t stream);
+int residual_norm(const nd_residual_norm_args& a, cudaStream_t stream);
+int quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq,
+                  float* scale, cudaStream_t stream);
+int linear_w8a8(const nd_linear_w8a8_args& a, cudaStream_t stream);
 int gemv(const nd_gemv_args& a, cudaStream_t stream);
 int gemv_w8(const nd_gemv_args& a, cudaStream_t stream);
 int quantize_weights(const void* src, int src_dtype, int64_t rows, int64_t cols, int64_t group,

@@ -259,6 +259,21 @@ int nd_op_rmsnorm(const nd_rmsnorm_args* args, void* stream) {
   return nd::rmsnorm(*args, static_cast<cudaStream_t>(stream));
 }
 
+int nd_op_residual_norm(const nd_residual_norm_args* args, void* stream) {
+  if (!args) return nd::fail(ND_ERR_INVALID, "nd_op_residual_norm: null args");
+  return nd::residual_norm(*args, static_cast<cudaStream_t>(stream));
+}
+
+int nd_op_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq,
+                        float* scale, void* stream) {
+  return nd::quantize_rows(x, dtype, rows, cols, ldx, q, ldq, scale, static_cast<cudaStream_t>(stream));
+}
+
+int nd_op_linear_w8a8(const nd_linear_w8a8_args* args, void* stream) {
+  if (!args) return nd::fail(ND_ERR_INVALID, "nd_op_linear_w8a8: null args");
+  return nd::linear_w8a8(*args, static_cast<cudaStream_t>(stream));
+}
+
 int nd_op_gemv(const nd_gemv_args* args, void* stream) {
   if (!args) return nd::fail(ND_ERR_INVALID, "nd_op_gemv: null args");
   return nd::gemv(*args, static_cast<cudaStream_t>(stream));

@@ -13,9 +13,12 @@ import ctypes as C
 import torch
 
 from . import _lib
-from ._lib import AttentionArgs, GemvArgs, LinearArgs, ModulateArgs, RmsNormArgs, check, lib
+from ._lib import (AttentionArgs, GemvArgs, LinearArgs, LinearW8A8Args, ModulateArgs, ResidualNormArgs, RmsNormArgs,
+                   check, lib)
 
 _DT = {torch.bfloat16: _lib.ND_BF16, torch.float16: _lib.ND_F16, torch.float32: _lib.ND_F32}
+_DT8 = {**_DT, torch.int8: _lib.ND_I8}
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -224,6 +227,182 @@ def modulate(x: torch.Tensor, shift: torch.Tensor | None, scale: torch.Tensor, *
     a.eps = eps
     check(lib().nd_op_modulate(C.byref(a), C.c_void_p(_stream())))
     return out
+
+
+def _ld(t: torch.Tensor, multiple: int = 1) -> int:
+    """The row stride of a matrix; a single row's is never used and may be anything."""
+    return t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // multiple) * multiple
+
+
+def _padded(rows: int, cols: int, multiple: int, device, dtype) -> torch.Tensor:
+    """An uninitialised [rows, cols] matrix whose row stride is a multiple of `multiple`."""
+    wide = -(-cols // multiple) * multiple
+    t = torch.empty(rows, wide, device=device, dtype=dtype)
+    return t if wide == cols else t[:, :cols]
+
+
+def _check_matrix(what: str, t: torch.Tensor, dtypes, device) -> None:
+    if t.dim() != 2 or t.dtype not in dtypes or t.device != device or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{what} must be a 2-D {'/'.join(str(d) for d in dtypes)} tensor with unit column stride on "
+                         f"{device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+
+
+def _launch(what: str, device, fn, *args) -> None:
+    """Call an op on the current stream of the tensors' device."""
+    if device.type != "cuda":
+        raise ValueError(f"{what}: the tensors must be on a CUDA device, got {device}")
+    if device.index == torch.cuda.current_device():
+        check(fn(*args, C.c_void_p(torch.cuda.current_stream(device).cuda_stream)))
+        return
+    with torch.cuda.device(device):
+        check(fn(*args, C.c_void_p(torch.cuda.current_stream(device).cuda_stream)))
+
+
+def residual_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *, x_out: torch.Tensor | None = None,
+                  post_norm: int = _lib.ND_NORM_NONE, post_weight: torch.Tensor | None = None,
+                  gate: torch.Tensor | None = None, residual_scale: float = 1.0,
+                  pre_norm: int = _lib.ND_NORM_LAYER, pre_weight: torch.Tensor | None = None,
+                  scale: torch.Tensor | None = None, shift: torch.Tensor | None = None, rows_per_vec: int = 0,
+                  plus_one: bool = False, eps: float = 1e-6, out_dtype=torch.bfloat16,
+                  out: torch.Tensor | None = None, out_scale: torch.Tensor | None = None):
+    """x' = residual_scale * x + gate * post(branch), then y = pre(x') * (1 + scale) + shift, in one pass.
+
+    x: fp32 [rows, width], updated in place unless x_out is given (without a
+    branch and a residual_scale x' is x, and is only stored into x_out).
+    post_norm / pre_norm: ND_NORM_NONE, _RMS or _LAYER, times post_weight /
+    pre_weight [width] (+ 1 with plus_one). gate, scale, shift: [width], or
+    [vecs, width] of one row stride: row r reads set min(r // rows_per_vec,
+    vecs - 1). out_dtype None: x' only; torch.int8: one scale per row.
+    Returns (x', y), (x', q, y_scale) for int8, or (x', None).
+    """
+    _check_matrix("residual_norm: x", x, (torch.float32,), x.device)
+    rows, width = x.shape
+    device = x.device
+    if branch is not None:
+        _check_matrix("residual_norm: branch", branch, _FLOATS, device)
+        if tuple(branch.shape) != (rows, width):
+            raise ValueError(f"residual_norm: branch must be [{rows}, {width}], got {tuple(branch.shape)}")
+    _check_vec("residual_norm: post_weight", post_weight, width, device)
+    _check_vec("residual_norm: pre_weight", pre_weight, width, device)
+    vecs, stride = 1, width
+    sets = [(n, t) for n, t in (("gate", gate), ("scale", scale), ("shift", shift)) if t is not None]
+    if sets:
+        first = sets[0][1]
+        vecs = 1 if first.dim() == 1 else first.shape[0]
+        stride = first.stride(0) if vecs > 1 else width
+        for name, t in sets:
+            if (t.dim() not in (1, 2) or t.shape[-1] != width or (width > 1 and t.stride(-1) != 1)
+                    or t.dtype != torch.float32 or t.device != device or (1 if t.dim() == 1 else t.shape[0]) != vecs
+                    or (vecs > 1 and t.stride(0) != stride)):
+                raise ValueError(f"residual_norm: {name} must be float32 [{width}] or [vecs, {width}] on {device}, with "
+                                 f"the others' number of sets and row stride, got {tuple(t.shape)} {t.dtype}")
+    if vecs > 1 and rows_per_vec <= 0:
+        raise ValueError("residual_norm: several vector sets need rows_per_vec")
+    if x_out is not None:
+        _check_out("residual_norm: x_out", x_out, rows, width, (torch.float32,), device)
+    elif branch is not None or residual_scale != 1.0:
+        x_out = x
+    if out is not None:
+        _check_out("residual_norm: out", out, rows, width, (*_FLOATS, torch.int8), device)
+        out_dtype = out.dtype
+    elif out_dtype is not None:
+        if out_dtype not in _DT8:
+            raise ValueError(f"residual_norm: out_dtype must be a float type, torch.int8 or None, got {out_dtype}")
+        out = _padded(rows, width, 16 if out_dtype == torch.int8 else 1, device, out_dtype)
+    int8 = out_dtype == torch.int8
+    if int8:
+        if out_scale is None:
+            out_scale = torch.empty(rows, device=device, dtype=torch.float32)
+        else:
+            _check_vec("residual_norm: out_scale", out_scale, rows, device)
+    elif out_scale is not None:
+        raise ValueError("residual_norm: out_scale goes with an int8 output")
+    a = ResidualNormArgs(rows, width, x.data_ptr(), _ld(x), _ptr(x_out), _ld(x_out) if x_out is not None else 0,
+                         _ptr(branch), _ld(branch) if branch is not None else 0,
+                         _DT[branch.dtype] if branch is not None else 0, post_norm, _ptr(post_weight), _ptr(gate),
+                         residual_scale, pre_norm, _ptr(pre_weight), _ptr(scale), _ptr(shift), vecs, stride,
+                         rows_per_vec, int(plus_one), eps, _ptr(out), _ld(out) if out is not None else 0,
+                         _DT8[out_dtype] if out is not None else 0, _ptr(out_scale))
+    _launch("residual_norm", device, lib().nd_op_residual_norm, C.byref(a))
+    x_new = x if x_out is None else x_out
+    return (x_new, out, out_scale) if int8 else (x_new, out)
+
+
+def quantize_rows(x: torch.Tensor, *, out: torch.Tensor | None = None,
+                  scale: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows (tokens) as int8 with one scale each: scale = max |x| / 127 over the row, q = rint(x * 127 / max |x|),
+    the quotient rounded as if exact. Returns (q [rows, cols], scale [rows]); q's rows are a multiple of 16 bytes
+    apart, as linear_w8a8 reads them. A row with an infinity or a NaN gets scale NaN and q 0."""
+    _check_matrix("quantize_rows: x", x, _FLOATS, x.device)
+    rows, cols = x.shape
+    if out is None:
+        out = _padded(rows, cols, 16, x.device, torch.int8)
+    else:
+        _check_out("quantize_rows: out", out, rows, cols, (torch.int8,), x.device)
+    if scale is None:
+        scale = torch.empty(rows, device=x.device, dtype=torch.float32)
+    else:
+        _check_vec("quantize_rows: scale", scale, rows, x.device)
+    _launch("quantize_rows", x.device, lib().nd_op_quantize_rows, x.data_ptr(), _DT[x.dtype], rows, cols, _ld(x),
+            out.data_ptr(), _ld(out), scale.data_ptr())
+    return out, scale
+
+
+def linear_w8a8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, w_scale: torch.Tensor,
+                bias: torch.Tensor | None = None, *, epilogue: int = _lib.ND_EPI_STORE, out_dtype=torch.bfloat16,
+                out: torch.Tensor | None = None, residual: torch.Tensor | None = None,
+                gate: torch.Tensor | None = None, group_split: int | None = None, shared_weights: bool = False,
+                addend: torch.Tensor | None = None) -> torch.Tensor:
+    """epilogue(x_scale[r] * w_scale[c] * (x . W^T) + bias) with int8 x and int8 weight, the sum exact.
+
+    x [rows, in] and x_scale [rows] as quantize_rows or residual_norm write
+    them; weight [groups * out, in] int8 (row stride a multiple of 16) with
+    w_scale, one per weight row (quantize(w, quant_group=0,
+    scale_dtype=torch.float32)). rows >= group_split use the second group of
+    weight rows, or with shared_weights only the second bias / gate. Residual
+    epilogues update `residual` (fp32) in place and return it; STORE_F32 makes
+    one if none is given. SWIGLU / GEGLU: weight [2F, in], output [rows, F].
+    """
+    device = x.device
+    _check_matrix("linear_w8a8: x", x, (torch.int8,), device)
+    _check_matrix("linear_w8a8: weight", weight, (torch.int8,), device)
+    rows, k = x.shape
+    split = group_split is not None and group_split < rows
+    groups = 2 if split and not shared_weights else 1
+    gated = epilogue in (_lib.ND_EPI_SWIGLU, _lib.ND_EPI_GEGLU)
+    each = weight.shape[0] // groups
+    n = each // 2 if gated else each
+    if weight.shape[1] != k or each * groups != weight.shape[0] or (gated and each % 2):
+        raise ValueError(f"linear_w8a8: weight must be [{groups} * {'2 * ' if gated else ''}out, {k}], got {tuple(weight.shape)}")
+    _check_vec("linear_w8a8: x_scale", x_scale, rows, device)
+    _check_vec("linear_w8a8: w_scale", w_scale, weight.shape[0], device)
+    _check_vec("linear_w8a8: bias", bias, (2 if split else 1) * each, device)
+    _check_vec("linear_w8a8: gate", gate, (2 if split else 1) * n, device)
+    if epilogue in (_lib.ND_EPI_RESIDUAL_GATE, _lib.ND_EPI_RESIDUAL_ADD, _lib.ND_EPI_STORE_F32):
+        if residual is not None:
+            _check_out("linear_w8a8: residual", residual, rows, n, (torch.float32,), device)
+        elif epilogue == _lib.ND_EPI_STORE_F32:
+            residual = _padded(rows, n, 4, device, torch.float32)
+        else:
+            raise ValueError("linear_w8a8: this epilogue adds to residual, and none is given")
+        out, out_dtype = None, torch.bfloat16
+    elif out is not None:
+        _check_out("linear_w8a8: out", out, rows, n, (torch.float16, torch.bfloat16), device)
+        out_dtype, residual = out.dtype, None
+    else:
+        if out_dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"linear_w8a8: out_dtype must be float16 or bfloat16 (STORE_F32 for fp32), got {out_dtype}")
+        out, residual = _padded(rows, n, 8, device, out_dtype), None
+    if addend is not None:
+        _check_out("linear_w8a8: addend", addend, rows, n, (out_dtype,), device)
+    a = LinearW8A8Args(_DT[out_dtype], epilogue, rows, k, n, x.data_ptr(), _ld(x, 16), x_scale.data_ptr(),
+                       weight.data_ptr(), _ld(weight, 16), w_scale.data_ptr(), _ptr(bias),
+                       group_split if group_split is not None else rows, int(shared_weights),
+                       _ptr(out), _ld(out, 8) if out is not None else 0,
+                       _ptr(residual), _ld(residual, 4) if residual is not None else 0,
+                       _ptr(gate), 0, _ptr(addend), _ld(addend, 8) if addend is not None else 0)
+    _launch("linear_w8a8", device, lib().nd_op_linear_w8a8, C.byref(a))
+    return out if residual is None else residual
 
 
 def rmsnorm(x: torch.Tensor, weight: torch.Tensor | None, *, out_dtype=None, plus_one=False,
