@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <climits>
 
+#include "gemm2_i8_sm100.cuh"
 #include "gemm_i8_sm100.cuh"
 #include "nd_internal.h"
 #include "nd_runtime.h"
@@ -27,6 +28,45 @@ int launch_i8(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& t
   }
   const int tiles = ((g.M + 127) / 128) * ((g.N + BN - 1) / BN);
   ND_CUDA(launch_pdl(kernel, dim3(tiles), dim3(192), L::kLaunchBytes, stream, ta, tb, tc, g));
+  ND_CUDA(cudaGetLastError());
+  return ND_OK;
+}
+
+// The pair kernel: clusters of two CTAs, as many pairs as fit on the GPU at
+// once (looked up once per device), each looping over 256-row tiles.
+template <int BN, int STAGES>
+int launch_i8_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const I8GemmArgs& g,
+                   cudaStream_t stream) {
+  using L = I8PairSmem<BN, STAGES>;
+  auto kernel = gemm2_i8_sm100_kernel<BN, STAGES>;
+  static int max_pairs[64] = {};
+  int dev = 0;
+  ND_CUDA(cudaGetDevice(&dev));
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.blockDim = dim3(kI8PairThreads);
+  cfg.dynamicSmemBytes = L::kLaunchBytes;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  if (!max_pairs[dev & 63]) {
+    ND_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kLaunchBytes));
+    cfg.gridDim = dim3(2 * sm_count());
+    cfg.numAttrs = 1;
+    int n = 0;
+    ND_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+    if (n <= 0) return fail(ND_ERR_UNSUPPORTED, "linear_w8a8: no CTA pair fits on this GPU");
+    max_pairs[dev & 63] = n;
+  }
+  const int tiles = ((g.M + 255) / 256) * ((g.N + BN - 1) / BN);
+  cfg.gridDim = dim3(2 * std::min(tiles, max_pairs[dev & 63]));
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  ND_CUDA(cudaLaunchKernelEx(&cfg, kernel, ta, tb, tc, g));
   ND_CUDA(cudaGetLastError());
   return ND_OK;
 }
@@ -97,6 +137,14 @@ int linear_w8a8(const nd_linear_w8a8_args& a, cudaStream_t stream) {
   if (resid) rc = make_tmap_2d_typed(&tc, a.residual, ND_F32, a.rows, a.out_features, a.ldr, 32, 32, 128);
   else rc = make_tmap_2d_typed(&tc, a.y, a.dtype, a.rows, a.out_features, a.ldy, 32, 32, 64);
   if (rc) return rc;
+  const int64_t pair_tiles = ((a.rows + 255) / 256) * ((n_all + 255) / 256);
+  const bool pair_groups = !split || shared || a.group_split % 256 == 0;
+  if (a.rows >= 512 && pair_groups && 2 * pair_tiles >= sm_count() / 2) {
+    g.idesc = make_idesc_i8(256, 256);
+    rc = make_tmap_2d(&tb, a.weight, 1, groups * n_all, a.in_features, ldw, 128, 128, true);
+    if (rc) return rc;
+    return launch_i8_pair<256, 5>(ta, tb, tc, g, stream);
+  }
   constexpr int bn = 128;
   g.idesc = make_idesc_i8(128, bn);
   rc = make_tmap_2d(&tb, a.weight, 1, groups * n_all, a.in_features, ldw, gated ? bn / 2 : bn, 128, true);
