@@ -34,8 +34,9 @@ struct I8PairSmem {
   static constexpr int kBBytes = (BN / 2) * 128;
   static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr int kTiles = STAGES * kStageBytes;
-  static constexpr int kEpiOffset = kTiles;  // 8 warps x 2 buffers x 4 KB
-  static constexpr int kBarOffset = kEpiOffset + 8 * 2 * 4096;
+  static constexpr int kEpiOffset = kTiles;  // 8 warps x 4 KB
+  static constexpr int kVecOffset = kEpiOffset + 8 * 4096;
+  static constexpr int kBarOffset = kVecOffset + 8 * kI8VecWords * 4;
   static constexpr int kNumBars = 2 * STAGES + 5;  // full[S], empty[S], acc_full[2], acc_empty[2], drain
   static constexpr int kMiscOffset = kBarOffset + kNumBars * 8;
   static constexpr int kTotal = kMiscOffset + 16;
@@ -187,7 +188,8 @@ __global__ void __launch_bounds__(kI8PairThreads, 1)
     // ------------------------------------------------------------ epilogue (both CTAs)
     const int ew = warp & 3;          // TMEM lane quarter
     const int side = (warp - 2) >> 2; // half of the tile's columns
-    const uint32_t buf0 = sbase + L::kEpiOffset + (warp - 2) * 2 * 4096;
+    const uint32_t buf = sbase + L::kEpiOffset + (warp - 2) * 4096;
+    const uint32_t vecs = sbase + L::kVecOffset + (warp - 2) * kI8VecWords * 4;
     const uint32_t acce_leader0 = mapa_shared(acce_bar(0), 0);
     const uint32_t acce_leader1 = mapa_shared(acce_bar(1), 0);
     const int width = args.half > 0 ? args.half : args.N;
@@ -200,21 +202,25 @@ __global__ void __launch_bounds__(kI8PairThreads, 1)
       pair_tile_coords(t, num_m2, num_n, mt2, nt);
       const int row0 = mt2 * 256 + static_cast<int>(rank) * 128 + ew * 32;
       const int wgroup = !args.shared_weights && mt2 * 256 >= args.group_split ? 1 : 0;
+      const I8Rows rows = i8_rows(args, wgroup, row0);
+      const int col0 = nt * per_tile + side * (per_tile / 2);
       const float sx = row0 + lane < args.M ? __ldg(args.x_scale + row0 + lane) : 0.f;
+      if (row0 < args.M) i8_stage_vectors(args, vecs, wgroup, rows, col0, lane);
       if (!mbar_wait(accf_bar(acc), (local >> 1) & 1, abort_flag, args.status, kStatusTimeoutEpilogue)) break;
       __syncwarp();
       tc_fence_after();
       const uint32_t tbase = tmem_base + (static_cast<uint32_t>(ew * 32) << 16) + acc * BN;
       if (row0 < args.M) {
 #pragma unroll 1
-        for (int c = side * (per_tile / 64); c < (side + 1) * (per_tile / 64); ++c) {
-          const int ocol = nt * per_tile + c * 32;
+        for (int c = 0; c < per_tile / 64; ++c) {
+          const int ocol = col0 + c * 32;
           if (ocol >= width) break;
+          const uint32_t at = tbase + side * (per_tile / 2) + c * 32;
           uint32_t r[32], r2[32];
-          tmem_ld32(tbase + c * 32, r);
-          if (args.half > 0) tmem_ld32(tbase + BN / 2 + c * 32, r2);
+          tmem_ld32(at, r);
+          if (args.half > 0) tmem_ld32(at + BN / 2, r2);
           tmem_ld_wait();
-          i8_chunk(args, &tmC, wgroup, row0, ocol, sx, r, r2, buf0, sb, lane);
+          i8_chunk(args, &tmC, rows, row0, ocol, c * 32, sx, r, r2, vecs, buf, sb, lane);
         }
       }
       tc_fence_before();

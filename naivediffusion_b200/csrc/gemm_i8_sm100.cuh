@@ -6,9 +6,9 @@
 // blocks (128-byte swizzle, 32 bytes of K per instruction); a k block does
 // twice the multiplications for the same bytes.
 //
-// The scales are applied to the finished sum in fp32: (float(sum) * sx) * sw,
-// three roundings (the conversion of a sum above 2^24 is one), then the bias
-// and the activation, then one rounding to the output type.
+// The scales are applied to the finished sum in fp32: fma(float(sum) * sw, sx,
+// bias), three roundings (the conversion of a sum above 2^24 is one), then the
+// activation, then one rounding to the output type.
 #pragma once
 
 #include "gemm_sm100.cuh"
@@ -50,97 +50,239 @@ __device__ __forceinline__ void umma_ss_i8(uint32_t d_tmem, uint64_t a_desc, uin
       : "memory");
 }
 
-// 32 values of a per-column vector from `col` on; columns at and past n read
-// as 0. Any alignment: a second weight group's vectors start wherever n puts
-// them.
-__device__ __forceinline__ void load_cols32(const float* src, int col, int n, float (&v)[32]) {
-  if (col + 32 <= n && (reinterpret_cast<uintptr_t>(src + col) & 15u) == 0) {
-    const float4* s = reinterpret_cast<const float4*>(src + col);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float4 t = __ldg(s + i);
-      v[4 * i] = t.x; v[4 * i + 1] = t.y; v[4 * i + 2] = t.z; v[4 * i + 3] = t.w;
+// ------------------------------------------------------------ epilogue
+// A warp's columns of the per-column vectors, staged in its own shared memory
+// while the tile's MMAs run (read from global memory per chunk, their latency
+// stood between every two chunks: 8192 x 2048 x 2048 took 14000 cycles per tile
+// instead of its MMAs' 8200):
+//   words [0, 128)    w_scale     (gated: the first factor's 64, then the second's)
+//   words [128, 256)  bias        (likewise)
+//   words [256, 384)  gate
+constexpr int kI8VecWords = 384;
+
+// Lane l's four of the warp's columns: columns col + 4 l .. of a plain tile;
+// gated, lanes 0..15 the first factor's columns, lanes 16..31 the second's.
+// Columns at and past n are 0. Any alignment: a second weight group's vectors
+// start wherever n puts them.
+__device__ __forceinline__ void i8_stage_cols(uint32_t dst, const float* src, int col, int n, int half, int lane) {
+  float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (src) {
+    int c = col + 4 * lane;
+    if (half > 0 && lane >= 16) {
+      src += half;
+      c -= 64;
     }
+    if (c + 4 <= n && (reinterpret_cast<uintptr_t>(src + c) & 15u) == 0) {
+      t = __ldg(reinterpret_cast<const float4*>(src + c));
+    } else {
+      if (c < n) t.x = __ldg(src + c);
+      if (c + 1 < n) t.y = __ldg(src + c + 1);
+      if (c + 2 < n) t.z = __ldg(src + c + 2);
+      if (c + 3 < n) t.w = __ldg(src + c + 3);
+    }
+  }
+  st_shared_v4(dst + lane * 16, __float_as_uint(t.x), __float_as_uint(t.y), __float_as_uint(t.z), __float_as_uint(t.w));
+}
+
+// A warp's place in the two bias / gate groups of shared weights: the group
+// of its rows, and whether the split falls between them (then each lane reads
+// its own group's bias and gate from global memory, and the staged ones are 0).
+struct I8Rows {
+  int bgroup;
+  bool mixed;
+};
+__device__ __forceinline__ I8Rows i8_rows(const I8GemmArgs& a, int wgroup, int row0) {
+  I8Rows r;
+  r.bgroup = a.shared_weights ? (row0 >= a.group_split ? 1 : 0) : wgroup;
+  r.mixed = a.shared_weights && row0 < a.group_split && row0 + 31 >= a.group_split;
+  return r;
+}
+
+// Stage the warp's vectors for output columns [col, col + 128) (gated: + 64).
+__device__ __forceinline__ void i8_stage_vectors(const I8GemmArgs& a, uint32_t vecs, int wgroup, const I8Rows& rows,
+                                                 int col, int lane) {
+  const int n = a.half > 0 ? a.half : a.N;
+  const float* bias = a.bias && !rows.mixed ? a.bias + static_cast<long long>(rows.bgroup) * a.bias_stride : nullptr;
+  __syncwarp();  // the previous tile's reads are done
+  i8_stage_cols(vecs, a.w_scale + static_cast<long long>(wgroup) * a.N, col, n, a.half, lane);
+  i8_stage_cols(vecs + 512, bias, col, n, a.half, lane);
+  if (a.epi == kEpiResidualGate)
+    i8_stage_cols(vecs + 1024, rows.mixed ? nullptr : a.gate + rows.bgroup * a.gate_stride, col, n, 0, lane);
+  __syncwarp();
+}
+
+__device__ __forceinline__ float2 as_float2(uint32_t a, uint32_t b) {
+  return make_float2(__uint_as_float(a), __uint_as_float(b));
+}
+
+// Sums -> fma(float(sum) * sw, sx, bias) for 32 columns of this lane's row;
+// `vecs` points at the first column's w_scale.
+__device__ __forceinline__ void i8_scaled(const uint32_t (&r)[32], float sx, uint32_t vecs, float2 (&v)[16]) {
+  const float2 sx2 = make_float2(sx, sx);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    uint32_t w[4], b[4];
+    ld_shared_v4(vecs + 16 * i, w[0], w[1], w[2], w[3]);
+    ld_shared_v4(vecs + 512 + 16 * i, b[0], b[1], b[2], b[3]);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float2 sum = make_float2(static_cast<float>(static_cast<int>(r[4 * i + 2 * j])),
+                                     static_cast<float>(static_cast<int>(r[4 * i + 2 * j + 1])));
+      v[2 * i + j] = ffma2(fmul2(sum, as_float2(w[2 * j], w[2 * j + 1])), sx2, as_float2(b[2 * j], b[2 * j + 1]));
+    }
+  }
+}
+
+// v (op) this lane's own 32 values in global memory, of which n exist: a
+// straddling warp's bias (add) and gate (multiply).
+template <bool MUL>
+__device__ __forceinline__ void i8_own(float2 (&v)[16], const float* own, int n) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const float f = i < n ? __ldg(own + i) : 0.f;
+    float& t = (i & 1) ? v[i >> 1].y : v[i >> 1].x;
+    t = MUL ? t * f : t + f;
+  }
+}
+
+// Activations to fp32 accuracy: exponentials and reciprocals on the SFU, a few
+// ulp (tanh.approx, which the 16-bit kernels use, is off by 2^-11 of a tanh
+// that 1 + tanh cancels for negative arguments). The .ftz forms: a result or
+// operand below 2^-126 counts as 0, where a sigmoid is 0 or 1 to fp32. Where
+// exp(-u) overflows the sigmoid is 0.
+__device__ __forceinline__ float fast_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+// sigmoid(u) given -u * log2(e).
+__device__ __forceinline__ float2 i8_sigmoid2(float2 t) {
+  const float2 d = fadd2(make_float2(fast_exp2(t.x), fast_exp2(t.y)), make_float2(1.f, 1.f));
+  return make_float2(fast_rcp(d.x), fast_rcp(d.y));
+}
+__device__ __forceinline__ float2 splat(float f) { return make_float2(f, f); }
+__device__ __forceinline__ float2 i8_silu(float2 x) { return fmul2(x, i8_sigmoid2(fmul2(x, splat(-kLog2e)))); }
+// x sigmoid(2 sqrt(2 / pi) (x + 0.044715 x^3))
+__device__ __forceinline__ float2 i8_gelu_tanh(float2 x) {
+  constexpr float c = -1.5957691216057308f * kLog2e;
+  return fmul2(x, i8_sigmoid2(fmul2(x, ffma2(fmul2(x, x), splat(0.044715f * c), splat(c)))));
+}
+// Exact GELU, x (1 + erf(x / sqrt 2)) / 2 = max(x, 0) - |x| erfc(|x| / sqrt 2) / 2,
+// with erfc(z) = (a1 t + .. + a5 t^5) exp(-z^2), t = 1 / (1 + p z): Abramowitz
+// and Stegun 7.1.26, off by at most 1.5e-7, the form the reference's
+// CpuMath.Gelu has. Half the instructions of erff.
+__device__ __forceinline__ float2 i8_gelu_erf(float2 x) {
+  const float2 ax = make_float2(fabsf(x.x), fabsf(x.y));
+  const float2 d = ffma2(ax, splat(0.3275911f * 0.70710678118654752f), splat(1.f));
+  const float2 t = make_float2(fast_rcp(d.x), fast_rcp(d.y));
+  float2 p = ffma2(t, splat(1.061405429f), splat(-1.453152027f));
+  p = ffma2(t, p, splat(1.421413741f));
+  p = ffma2(t, p, splat(-0.284496736f));
+  p = ffma2(t, p, splat(0.254829592f));
+  const float2 z = fmul2(fmul2(x, x), splat(-0.5f * kLog2e));
+  const float2 e = fmul2(fmul2(p, t), make_float2(fast_exp2(z.x), fast_exp2(z.y)));
+  return ffma2(fmul2(ax, splat(-0.5f)), e, make_float2(fmaxf(x.x, 0.f), fmaxf(x.y, 0.f)));
+}
+
+// One warp's [32 rows x 32 columns] chunk (lane = row) through its 4 KB of
+// staging to TMA, in the tensor map's swizzle: 16-bit chunks alternate
+// between two halves, fp32 ones take all of it.
+__device__ __forceinline__ void i8_emit(const CUtensorMap* tm, int kind, uint32_t buf, int& sb, int lane, int row0,
+                                        int col, const float2 (&v)[16]) {
+  if (kind == kEmitBf16 || kind == kEmitF16) {
+    buf += static_cast<uint32_t>(sb) * 2048u;
+    sb ^= 1;
+    if (lane == 0) bulk_wait_read<1>();
+    __syncwarp();
+    uint32_t p[16];
+    if (kind == kEmitF16) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) p[i] = pack_f16(v[i].x, v[i].y);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) p[i] = pack_bf16(v[i].x, v[i].y);
+    }
+    // 64-byte rows, 64B swizzle: 16-byte chunk c of row r at c ^ ((r >> 1) & 3).
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      st_shared_v4(buf + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4), p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
   } else {
+    if (lane == 0) bulk_wait_read<0>();
+    __syncwarp();
+    // 128-byte rows, 128B swizzle: 16-byte chunk c of row r at c ^ (r & 7).
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = (col + i < n) ? __ldg(src + col + i) : 0.f;
+    for (int c = 0; c < 8; ++c)
+      st_shared_v4(buf + lane * 128 + ((c ^ (lane & 7)) << 4), __float_as_uint(v[2 * c].x), __float_as_uint(v[2 * c].y),
+                   __float_as_uint(v[2 * c + 1].x), __float_as_uint(v[2 * c + 1].y));
   }
-}
-
-// Sums -> (float(sum) * sx) * sw + bias for 32 columns of this lane's row.
-__device__ __forceinline__ void i8_scaled(const I8GemmArgs& a, const uint32_t (&r)[32], float sx, const float* sw,
-                                          const float* bias, int col, int n, float (&v)[32]) {
-  float w[32];
-  load_cols32(sw, col, n, w);
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = static_cast<float>(static_cast<int>(r[i])) * sx * w[i];
-  if (bias) {
-    load_cols32(bias, col, n, w);
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] += w[i];
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    if (kind == kEmitAddF32) tma_reduce_add_2d(tm, buf, col, row0);
+    else tma_store_2d(tm, buf, col, row0);
+    bulk_commit();
   }
-}
-
-// Activations to fp32 accuracy: exponentials and reciprocals on the SFU,
-// a few ulp (the 16-bit kernels' tanh.approx is 2^-11 of tanh, which a large
-// negative argument multiplies).
-__device__ __forceinline__ float i8_sigmoid(float u) { return __fdividef(1.0f, 1.0f + __expf(-u)); }
-__device__ __forceinline__ float i8_silu(float x) {
-  // exp(-x) overflows below -88: x * 0 is the limit (-0), not -inf * 0.
-  return x * i8_sigmoid(x);
-}
-__device__ __forceinline__ float i8_gelu_tanh(float x) {
-  return x * i8_sigmoid(1.5957691216f * fmaf(0.044715f * x, x * x, x));
 }
 
 // One chunk of 32 output columns from `ocol`, rows row0 + lane: the sums `r`
 // (and, for the gated epilogues, the second factor's sums `r2`) through the
-// epilogue to the output's tensor map.
-__device__ __forceinline__ void i8_chunk(const I8GemmArgs& a, const CUtensorMap* tmC, int wgroup, int row0, int ocol,
-                                         float sx, const uint32_t (&r)[32], const uint32_t (&r2)[32], uint32_t buf0,
-                                         int& sb, int lane) {
+// epilogue to the output's tensor map. `vecs`: the warp's staged vectors, `lc`
+// the chunk's first column among them.
+__device__ __forceinline__ void i8_chunk(const I8GemmArgs& a, const CUtensorMap* tmC, const I8Rows& rows, int row0,
+                                         int ocol, int lc, float sx, const uint32_t (&r)[32], const uint32_t (&r2)[32],
+                                         uint32_t vecs, uint32_t buf, int& sb, int lane) {
   const int row = row0 + lane;
-  const int bgroup = a.shared_weights ? (row >= a.group_split ? 1 : 0) : wgroup;
-  const float* sw = a.w_scale + static_cast<long long>(wgroup) * a.N;
-  const float* bias = a.bias ? a.bias + static_cast<long long>(bgroup) * a.bias_stride : nullptr;
+  const bool second = row >= a.group_split;  // read by straddling warps only
   int kind = a.out_f16 ? kEmitF16 : kEmitBf16;
-  float v[32];
+  float2 v[16];
+  i8_scaled(r, sx, vecs + 4 * lc, v);
   if (a.half > 0) {
-    float g[32];
-    i8_scaled(a, r, sx, sw, bias, ocol, a.half, v);
-    i8_scaled(a, r2, sx, sw + a.half, bias ? bias + a.half : nullptr, ocol, a.half, g);
+    float2 g[16];
+    i8_scaled(r2, sx, vecs + 4 * (64 + lc), g);
+    if (rows.mixed && a.bias) {
+      const float* own = a.bias + (second ? a.bias_stride : 0) + ocol;
+      i8_own<false>(v, own, a.half - ocol);
+      i8_own<false>(g, own + a.half, a.half - ocol);
+    }
     if (a.epi == kEpiGeGlu) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] *= gelu_erf(g[i]);
+      for (int i = 0; i < 16; ++i) v[i] = fmul2(v[i], i8_gelu_erf(g[i]));
     } else {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = i8_silu(v[i]) * g[i];
+      for (int i = 0; i < 16; ++i) v[i] = fmul2(i8_silu(v[i]), g[i]);
     }
-    emit_chunk(tmC, kind, buf0, sb, lane, row0, a.M, ocol, v);
+    i8_emit(tmC, kind, buf, sb, lane, row0, ocol, v);
     return;
   }
-  i8_scaled(a, r, sx, sw, bias, ocol, a.N, v);
+  if (rows.mixed && a.bias) i8_own<false>(v, a.bias + (second ? a.bias_stride : 0) + ocol, a.N - ocol);
   switch (a.epi) {
     case kEpiGeluTanh:
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = i8_gelu_tanh(v[i]);
+      for (int i = 0; i < 16; ++i) v[i] = i8_gelu_tanh(v[i]);
       break;
     case kEpiGeluErf:
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = gelu_erf(v[i]);
+      for (int i = 0; i < 16; ++i) v[i] = i8_gelu_erf(v[i]);
       break;
     case kEpiSilu:
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = i8_silu(v[i]);
+      for (int i = 0; i < 16; ++i) v[i] = i8_silu(v[i]);
       break;
-    case kEpiResidualGate: {
-      float g[32];
-      load_cols32(a.gate + bgroup * a.gate_stride, ocol, a.N, g);
+    case kEpiResidualGate:
+      if (rows.mixed) {
+        i8_own<true>(v, a.gate + (second ? a.gate_stride : 0) + ocol, a.N - ocol);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] *= g[i];
+        for (int i = 0; i < 8; ++i) {
+          uint32_t g[4];
+          ld_shared_v4(vecs + 1024 + 4 * lc + 16 * i, g[0], g[1], g[2], g[3]);
+          v[2 * i] = fmul2(v[2 * i], as_float2(g[0], g[1]));
+          v[2 * i + 1] = fmul2(v[2 * i + 1], as_float2(g[2], g[3]));
+        }
+      }
       kind = kEmitAddF32;
       break;
-    }
     case kEpiResidualAdd:
       kind = kEmitAddF32;
       break;
@@ -154,8 +296,9 @@ __device__ __forceinline__ void i8_chunk(const I8GemmArgs& a, const CUtensorMap*
         for (int i = 0; i < 32; ++i) {
           if (ocol + i < a.N) {
             const uint16_t h = ad[i];
-            v[i] += a.out_f16 ? __half2float(*reinterpret_cast<const __half*>(&h))
-                              : __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(&h));
+            float& t = (i & 1) ? v[i >> 1].y : v[i >> 1].x;
+            t += a.out_f16 ? __half2float(*reinterpret_cast<const __half*>(&h))
+                           : __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(&h));
           }
         }
       }
@@ -163,7 +306,7 @@ __device__ __forceinline__ void i8_chunk(const I8GemmArgs& a, const CUtensorMap*
     default:
       break;
   }
-  emit_chunk(tmC, kind, buf0, sb, lane, row0, a.M, ocol, v);
+  i8_emit(tmC, kind, buf, sb, lane, row0, ocol, v);
 }
 
 template <int BN, int STAGES>
@@ -172,8 +315,9 @@ struct I8Smem {
   static constexpr int kBBytes = BN * 128;
   static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr int kTiles = STAGES * kStageBytes;
-  static constexpr int kEpiOffset = kTiles;  // 4 warps x 2 buffers x 4 KB
-  static constexpr int kBarOffset = kEpiOffset + 4 * 2 * 4096;
+  static constexpr int kEpiOffset = kTiles;  // 4 warps x 4 KB
+  static constexpr int kVecOffset = kEpiOffset + 4 * 4096;
+  static constexpr int kBarOffset = kVecOffset + 4 * kI8VecWords * 4;
   static constexpr int kNumBars = 2 * STAGES + 2;  // full[S], empty[S], acc_full, drain
   static constexpr int kMiscOffset = kBarOffset + kNumBars * 8;
   static constexpr int kTotal = kMiscOffset + 16;
@@ -301,12 +445,15 @@ __global__ void __launch_bounds__(192, 1)
   } else {
     const int ew = warp & 3;
     const int row0 = m0 + ew * 32;
-    const uint32_t buf0 = sbase + L::kEpiOffset + ew * 2 * 4096;
+    const uint32_t buf = sbase + L::kEpiOffset + ew * 4096;
+    const uint32_t vecs = sbase + L::kVecOffset + ew * kI8VecWords * 4;
+    const I8Rows rows = i8_rows(args, wgroup, row0);
+    const float sx = row0 + lane < args.M ? __ldg(args.x_scale + row0 + lane) : 0.f;
     int sb = 0;
+    if (row0 < args.M) i8_stage_vectors(args, vecs, wgroup, rows, nt * (args.half > 0 ? BN / 2 : BN), lane);
     if (row0 < args.M && mbar_wait(accf_bar, 0, abort_flag, args.status, kStatusTimeoutEpilogue)) {
       __syncwarp();
       tc_fence_after();
-      const float sx = row0 + lane < args.M ? __ldg(args.x_scale + row0 + lane) : 0.f;
       const uint32_t tbase = tmem_base + (static_cast<uint32_t>(ew * 32) << 16);
       const int width = args.half > 0 ? args.half : args.N;
       const int per_tile = args.half > 0 ? BN / 2 : BN;
@@ -318,7 +465,7 @@ __global__ void __launch_bounds__(192, 1)
         tmem_ld32(tbase + c * 32, r);
         if (args.half > 0) tmem_ld32(tbase + BN / 2 + c * 32, r2);
         tmem_ld_wait();
-        i8_chunk(args, &tmC, wgroup, row0, ocol, sx, r, r2, buf0, sb, lane);
+        i8_chunk(args, &tmC, rows, row0, ocol, c * 32, sx, r, r2, vecs, buf, sb, lane);
       }
       tc_fence_before();
     }

@@ -23,6 +23,9 @@ namespace nd {
 
 namespace {
 
+// The fast product x * (127 / peak) is off by at most 2^-23 * 127 = 1.5e-5.
+constexpr float kNearHalf = 0.49997f;
+
 // VEC values of type ND_F32 / ND_F16 / ND_BF16 as fp32.
 template <int VEC>
 __device__ __forceinline__ void load_vals(const void* p, long long i, int type, float (&f)[VEC]) {
@@ -54,26 +57,25 @@ __device__ __forceinline__ void load_vals(const void* p, long long i, int type, 
 }
 
 // The exact quotient's nearest integer, as bits whose low byte is q.
-__device__ __noinline__ uint32_t rint_exact(float x, float peak) {
+__device__ __forceinline__ uint32_t rint_exact(float x, float peak) {
   return static_cast<uint32_t>(__double2int_rn(__ddiv_rn(static_cast<double>(x) * 127.0, static_cast<double>(peak))));
 }
 
+// VEC values by the fast product; returns their largest distance from the
+// integer taken.
 template <int VEC>
-__device__ __forceinline__ void quantize_store(int8_t* q, const float (&f)[VEC], const RowScale& s) {
+__device__ __forceinline__ float quantize_store(int8_t* q, const float (&f)[VEC], float inverse) {
   uint32_t u[4] = {0u, 0u, 0u, 0u};
-  if (s.inverse != 0.f) {
-    const bool tiny = s.peak < 1e-30f;  // 127 / peak leaves fp32's range
-    float off[4] = {0.f, 0.f, 0.f, 0.f};
+  float most = 0.f;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) u[j] = rint_bits(f[j] * s.inverse, off[j]);
-    if (tiny || fmaxf(fmaxf(off[0], off[1]), fmaxf(off[2], off[3])) > 0.49997f) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j)
-        if (tiny || off[j] > 0.49997f) u[j] = rint_exact(f[j], s.peak);
-    }
+  for (int j = 0; j < VEC; ++j) {
+    float off;
+    u[j] = rint_bits(f[j] * inverse, off);
+    most = fmaxf(most, off);
   }
   if constexpr (VEC == 4) *reinterpret_cast<uint32_t*>(q) = pack_low_bytes(u[0], u[1], u[2], u[3]);
   else *q = static_cast<int8_t>(u[0] & 0xffu);
+  return most;
 }
 
 __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
@@ -117,15 +119,39 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* x, long 
   const RowScale s = row_scale(block_max(peak, red));
   if (threadIdx.x == 0) scale[r] = s.scale;
   int8_t* out = q + r * ldq;
+  if (s.inverse == 0.f) {  // zeros, or infinities and NaN: every q is 0
+    const float zero[VEC] = {};
+#pragma unroll 1
+    for (int c = threadIdx.x * VEC; c < width; c += blockDim.x * VEC) quantize_store<VEC>(out + c, zero, 0.f);
+    return;
+  }
+  float most = 0.f;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int c = (threadIdx.x + blockDim.x * i) * VEC;
-    if (c < width) quantize_store<VEC>(out + c, v[i], s);
+    if (c < width) most = fmaxf(most, quantize_store<VEC>(out + c, v[i], s.inverse));
   }
   for (int c = (threadIdx.x + blockDim.x * V) * VEC; c < width; c += blockDim.x * VEC) {
     float w[VEC];
     load_vals<VEC>(x, x0 + c, type, w);
-    quantize_store<VEC>(out + c, w, s);
+    most = fmaxf(most, quantize_store<VEC>(out + c, w, s.inverse));
+  }
+  // Rare (one thread in a few hundred): a value whose quotient may lie on the
+  // other side of a half, or a row whose 127 / peak leaves fp32's range. The
+  // thread's values are read again, out of the cache, and those divided.
+  const bool tiny = s.peak < 1e-30f;
+  if (tiny || most > kNearHalf) {
+#pragma unroll 1
+    for (int c = threadIdx.x * VEC; c < width; c += blockDim.x * VEC) {
+      float w[VEC];
+      load_vals<VEC>(x, x0 + c, type, w);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        float off;
+        rint_bits(w[j] * s.inverse, off);
+        if (tiny || off > kNearHalf) out[c + j] = static_cast<int8_t>(rint_exact(w[j], s.peak) & 0xffu);
+      }
+    }
   }
 }
 
