@@ -211,16 +211,30 @@ __global__ void __launch_bounds__(kI8PairThreads, 1)
       tc_fence_after();
       const uint32_t tbase = tmem_base + (static_cast<uint32_t>(ew * 32) << 16) + acc * BN;
       if (row0 < args.M) {
+        const uint32_t at = tbase + side * (per_tile / 2);
+        const int chunks = min(per_tile / 64, (width - col0 + 31) / 32);  // may be <= 0
+        if (args.half > 0) {
 #pragma unroll 1
-        for (int c = 0; c < per_tile / 64; ++c) {
-          const int ocol = col0 + c * 32;
-          if (ocol >= width) break;
-          const uint32_t at = tbase + side * (per_tile / 2) + c * 32;
-          uint32_t r[32], r2[32];
+          for (int c = 0; c < chunks; ++c) {
+            uint32_t r[32], r2[32];
+            tmem_ld32(at + c * 32, r);
+            tmem_ld32(at + BN / 2 + c * 32, r2);
+            tmem_ld_wait();
+            i8_chunk(args, &tmC, rows, row0, col0 + c * 32, c * 32, sx, r, r2, vecs, buf, sb, lane);
+          }
+        } else if (chunks > 0) {
+          // The next chunk's sums are on their way while this one is worked on.
+          uint32_t r[32], next[32];
           tmem_ld32(at, r);
-          if (args.half > 0) tmem_ld32(at + BN / 2, r2);
           tmem_ld_wait();
-          i8_chunk(args, &tmC, rows, row0, ocol, c * 32, sx, r, r2, vecs, buf, sb, lane);
+#pragma unroll 1
+          for (int c = 0; c < chunks; ++c) {
+            if (c + 1 < chunks) tmem_ld32(at + (c + 1) * 32, next);
+            i8_chunk(args, &tmC, rows, row0, col0 + c * 32, c * 32, sx, r, r, vecs, buf, sb, lane);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = next[i];
+          }
         }
       }
       tc_fence_before();
