@@ -186,10 +186,10 @@ def lib() -> C.CDLL:
         L.nd_op_rmsnorm.argtypes = [C.POINTER(RmsNormArgs), C.c_void_p]
         L.nd_op_head_norm_rope.argtypes = [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int, C.c_int, C.c_void_p,
                                            C.c_void_p, C.c_void_p, C.c_float, C.c_void_p]
-        L.nd_op_residual_norm.argtypes = [C.POINTER(ResidualNormArgs), C.c_void_p]
+        L.nd_op_residual_norm.argtypes = [C.c_void_p, C.c_void_p]  # ResidualNormArgs, or its packed bytes
         L.nd_op_quantize_rows.argtypes = [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_void_p,
                                           C.c_int64, C.c_void_p, C.c_void_p]
-        L.nd_op_linear_w8a8.argtypes = [C.POINTER(LinearW8A8Args), C.c_void_p]
+        L.nd_op_linear_w8a8.argtypes = [C.c_void_p, C.c_void_p]    # LinearW8A8Args, likewise
         L.nd_op_gemv.argtypes = [C.POINTER(GemvArgs), C.c_void_p]
         L.nd_op_patchify.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int,
                                      C.c_int, C.c_int, C.c_int64, C.c_void_p]

@@ -4,7 +4,9 @@
 #include <climits>
 
 #include "gemm2_i8_sm100.cuh"
+#include "gemm_i8_few_sm100.cuh"
 #include "gemm_i8_sm100.cuh"
+#include "gemv_i8.cuh"
 #include "nd_internal.h"
 #include "nd_runtime.h"
 
@@ -12,24 +14,91 @@ namespace nd {
 
 namespace {
 
+constexpr int kMaxSplits = 8;  // the portable cluster size
+constexpr int kFewRows = 32;   // of gemm_i8_few_kernel
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Launch a kernel whose clusters of S CTAs share a tile's k blocks. A k block
+// takes block_us on one SM (both kernels run at the rate an SM takes bytes
+// from L2, about 106 GB/s), and a split costs fixed_us + S * each_us for the
+// cluster barriers and the sums' way through the cluster's shared memory
+// (measured per kernel). S is the cheapest count whose clusters all run at
+// once (`most`, looked up once per kernel and device).
+struct SplitCost {
+  float block_us, fixed_us, each_us;
+};
+template <typename Kernel, typename... Args>
+int launch_split(Kernel kernel, int* most, int smem, int tiles, int num_kb, SplitCost c, cudaStream_t stream,
+                 const Args&... args) {
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.blockDim = dim3(192);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  if (!most[1]) {
+    ND_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    cfg.numAttrs = 1;
+    for (int s = kMaxSplits; s >= 1; --s) {
+      attr[0].val.clusterDim.x = s;
+      cfg.gridDim = dim3(s * sm_count());
+      int n = 0;
+      ND_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+      most[s] = std::max(n, 1);
+    }
+  }
+  int splits = 1;
+  float best = c.block_us * num_kb;
+  for (int s = 2; s <= std::min(kMaxSplits, num_kb); ++s) {
+    const float cost = c.block_us * ((num_kb + s - 1) / s) + c.fixed_us + c.each_us * s;
+    if (tiles <= most[s] && cost < best) {
+      best = cost;
+      splits = s;
+    }
+  }
+  attr[0].val.clusterDim.x = splits;
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles) * splits);
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  ND_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+  ND_CUDA(cudaGetLastError());
+  return ND_OK;
+}
+
+int current_device(int* dev) {
+  ND_CUDA(cudaGetDevice(dev));
+  return ND_OK;
+}
+
+// The one-SM kernel: 128 x BN tiles.
 template <int BN, int STAGES>
 int launch_i8(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const I8GemmArgs& g,
               cudaStream_t stream) {
   using L = I8Smem<BN, STAGES>;
-  auto kernel = gemm_i8_sm100_kernel<BN, STAGES>;
-  static bool configured[64] = {};
+  static int most[64][kMaxSplits + 1] = {};
   int dev = 0;
-  ND_CUDA(cudaGetDevice(&dev));
-  if (!configured[dev & 63]) {
-    ND_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kLaunchBytes));
-    configured[dev & 63] = true;
-  }
+  if (int rc = current_device(&dev)) return rc;
   const int tiles = ((g.M + 127) / 128) * ((g.N + BN - 1) / BN);
-  ND_CUDA(launch_pdl(kernel, dim3(tiles), dim3(192), L::kLaunchBytes, stream, ta, tb, tc, g));
-  ND_CUDA(cudaGetLastError());
-  return ND_OK;
+  const float quarters = static_cast<float>(std::min(4, (g.M + 31) / 32));  // of a tile's rows that exist: what is summed
+  return launch_split(gemm_i8_sm100_kernel<BN, STAGES>, most[dev & 63], L::kLaunchBytes, tiles, (g.K + 127) / 128,
+                      SplitCost{0.165f, 0.1f * quarters, 0.3f * quarters}, stream, ta, tb, tc, g);
+}
+
+// The kernel for few rows: 128 weight rows x NT tokens.
+template <int NT, int STAGES>
+int launch_i8_few(const CUtensorMap& tw, const CUtensorMap& tx, const I8FewArgs& g, cudaStream_t stream) {
+  using L = I8FewSmem<NT, STAGES>;
+  static int most[64][kMaxSplits + 1] = {};
+  int dev = 0;
+  if (int rc = current_device(&dev)) return rc;
+  const int tiles = g.g.half > 0 ? g.g.half / 64 : (g.g.N + 127) / 128;
+  return launch_split(gemm_i8_few_kernel<NT, STAGES>, most[dev & 63], L::kLaunchBytes, tiles, (g.g.K + 127) / 128,
+                      SplitCost{0.17f, 0.f, 0.25f}, stream, tw, tx, g);
 }
 
 // The pair kernel: clusters of two CTAs, as many pairs as fit on the GPU at
@@ -67,6 +136,40 @@ int launch_i8_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorM
   cfg.gridDim = dim3(2 * std::min(tiles, max_pairs[dev & 63]));
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
   ND_CUDA(cudaLaunchKernelEx(&cfg, kernel, ta, tb, tc, g));
+  ND_CUDA(cudaGetLastError());
+  return ND_OK;
+}
+
+// Pair or one-SM kernel. A k block of either takes an SM its 32 KB at the rate
+// it takes bytes from L2, 0.30 us, for a 128 x 256 share of a pair tile or
+// for a 128 x 128 tile (whose missing rows cost nothing); what counts is the
+// number of rounds.
+bool pair_is_faster(int64_t rows, int64_t n) {
+  const int sms = sm_count();
+  const int64_t pair_tiles = ((rows + 255) / 256) * ((n + 255) / 256), tiles = ((rows + 127) / 128) * ((n + 127) / 128);
+  const int64_t pair_rounds = (pair_tiles + sms / 2 - 1) / (sms / 2), rounds = (tiles + sms - 1) / sms;
+  const float real = rows < 128 ? rows / 128.f : 1.f;
+  return pair_rounds < rounds * (0.5f + 0.5f * real);
+}
+
+int launch_i8_gemv(const nd_linear_w8a8_args& a, const I8GemmArgs& g, int64_t ldw, bool resid, cudaStream_t stream) {
+  I8GemvArgs v{};
+  v.g = g;
+  v.x = a.x;
+  v.w = a.weight;
+  v.ldx = a.ldx;
+  v.ldw = ldw;
+  v.y = a.y;
+  v.residual = a.residual;
+  v.ld = resid ? a.ldr : a.ldy;
+  const int warps = g.half > 0 ? g.half : (g.N + 1) / 2;
+  const dim3 grid((warps + kGemvI8Threads / 32 - 1) / (kGemvI8Threads / 32));
+  switch (g.M) {
+    case 1: ND_CUDA(launch_pdl(gemv_i8_kernel<1>, grid, dim3(kGemvI8Threads), 0, stream, v)); break;
+    case 2: ND_CUDA(launch_pdl(gemv_i8_kernel<2>, grid, dim3(kGemvI8Threads), 0, stream, v)); break;
+    case 3: ND_CUDA(launch_pdl(gemv_i8_kernel<3>, grid, dim3(kGemvI8Threads), 0, stream, v)); break;
+    default: ND_CUDA(launch_pdl(gemv_i8_kernel<4>, grid, dim3(kGemvI8Threads), 0, stream, v)); break;
+  }
   ND_CUDA(cudaGetLastError());
   return ND_OK;
 }
@@ -131,15 +234,34 @@ int linear_w8a8(const nd_linear_w8a8_args& a, cudaStream_t stream) {
   g.status = device_status();
   if (!g.status) return fail(ND_ERR_CUDA, "linear_w8a8: no device status word");
 
+  if (a.rows <= kGemvI8Rows) return launch_i8_gemv(a, g, ldw, resid, stream);
+
   CUtensorMap ta, tb, tc;
+  if (a.rows <= kFewRows) {
+    const int nt = a.rows <= 16 ? 16 : 32;
+    int rc = make_tmap_2d(&ta, a.weight, 1, n_all, a.in_features, ldw, gated ? 16 : 128, 128, true);
+    if (rc) return rc;
+    rc = make_tmap_2d(&tb, a.x, 1, a.rows, a.in_features, a.ldx, nt, 128, true);
+    if (rc) return rc;
+    I8FewArgs f{};
+    f.g = g;
+    f.g.idesc = make_idesc_i8(128, nt);
+    f.y = a.y;
+    f.residual = a.residual;
+    f.ld = resid ? a.ldr : a.ldy;
+    // More tiles than SMs: half the stages, so that two CTAs share an SM and
+    // one's loads run under the other's start and end.
+    const bool two = (gated ? a.out_features / 64 : (n_all + 127) / 128) > sm_count();
+    if (nt == 16) return two ? launch_i8_few<16, 6>(ta, tb, f, stream) : launch_i8_few<16, 12>(ta, tb, f, stream);
+    return two ? launch_i8_few<32, 5>(ta, tb, f, stream) : launch_i8_few<32, 11>(ta, tb, f, stream);
+  }
   int rc = make_tmap_2d(&ta, a.x, 1, a.rows, a.in_features, a.ldx, 128, 128, true);
   if (rc) return rc;
   if (resid) rc = make_tmap_2d_typed(&tc, a.residual, ND_F32, a.rows, a.out_features, a.ldr, 32, 32, 128);
   else rc = make_tmap_2d_typed(&tc, a.y, a.dtype, a.rows, a.out_features, a.ldy, 32, 32, 64);
   if (rc) return rc;
-  const int64_t pair_tiles = ((a.rows + 255) / 256) * ((n_all + 255) / 256);
   const bool pair_groups = !split || shared || a.group_split % 256 == 0;
-  if (a.rows >= 512 && pair_groups && 2 * pair_tiles >= sm_count() / 2) {
+  if (pair_groups && pair_is_faster(a.rows, n_all)) {
     g.idesc = make_idesc_i8(256, 256);
     rc = make_tmap_2d(&tb, a.weight, 1, groups * n_all, a.in_features, ldw, 128, 128, true);
     if (rc) return rc;

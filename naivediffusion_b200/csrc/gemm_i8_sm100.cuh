@@ -11,7 +11,7 @@
 // activation, then one rounding to the output type.
 #pragma once
 
-#include "gemm_sm100.cuh"
+#include "gemm2_sm100.cuh"
 
 namespace nd {
 
@@ -324,8 +324,25 @@ struct I8Smem {
   static constexpr int kLaunchBytes = kTotal + 1024;
 };
 
-// One 128 x BN tile per CTA. 192 threads: warp 0 loads, warp 1 issues the
-// MMAs, warps 2..5 are the epilogue (warp w reads TMEM lanes 32 (w % 4) on).
+__device__ __forceinline__ uint32_t cluster_nctas() {
+  uint32_t n;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ int ld_shared_cluster(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// One 128 x BN tile per cluster of S CTAs, S = 1 where the tiles fill the GPU.
+// With few tiles the k blocks are split over the cluster: each CTA sums its
+// share, leaves its integer sums in its own shared memory (columns of 128
+// rows, where the operand tiles were), and after a cluster barrier the tile's
+// [32 x 32] chunks are divided over the CTAs, each chunk added up from all S
+// shared memories. Integer sums: the split changes no bit, and nothing goes
+// through global memory. 192 threads: warp 0 loads, warp 1 issues the MMAs,
+// warps 2..5 are the epilogue (warp w reads TMEM lanes 32 (w % 4) on).
 template <int BN, int STAGES>
 __global__ void __launch_bounds__(192, 1)
     gemm_i8_sm100_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -347,9 +364,13 @@ __global__ void __launch_bounds__(192, 1)
   const int lane = threadIdx.x & 31;
   const int num_m = (args.M + 127) / 128;
   const int num_n = (args.N + BN - 1) / BN;
-  const int num_kb = (args.K + 127) / 128;
+  const int splits = static_cast<int>(cluster_nctas());
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int all_kb = (args.K + 127) / 128;
+  const int kb0 = all_kb * rank / splits;  // this CTA's k blocks: at least one, the host sees to it
+  const int num_kb = all_kb * (rank + 1) / splits - kb0;
   int mt, nt;
-  tile_coords(blockIdx.x, num_m, num_n, mt, nt);
+  tile_coords(blockIdx.x / splits, num_m, num_n, mt, nt);
   const int m0 = mt * 128;
   const int wgroup = !args.shared_weights && m0 >= args.group_split ? 1 : 0;
 
@@ -392,13 +413,14 @@ __global__ void __launch_bounds__(192, 1)
         const uint32_t a_dst = sbase + stage * L::kStageBytes;
         const uint32_t b_dst = a_dst + L::kABytes;
         mbar_arrive_expect_tx(full_bar(stage), L::kStageBytes);
-        tma_load_2d(a_dst, &tmA, full_bar(stage), kb * 128, m0);
+        const int k0 = (kb0 + kb) * 128;
+        tma_load_2d(a_dst, &tmA, full_bar(stage), k0, m0);
         if (args.half > 0) {
-          tma_load_2d(b_dst, &tmB, full_bar(stage), kb * 128, wgroup * args.N + nt * (BN / 2));
-          tma_load_2d(b_dst + (BN / 2) * 128, &tmB, full_bar(stage), kb * 128,
+          tma_load_2d(b_dst, &tmB, full_bar(stage), k0, wgroup * args.N + nt * (BN / 2));
+          tma_load_2d(b_dst + (BN / 2) * 128, &tmB, full_bar(stage), k0,
                       wgroup * args.N + args.half + nt * (BN / 2));
         } else {
-          tma_load_2d(b_dst, &tmB, full_bar(stage), kb * 128, wgroup * args.N + nt * BN);
+          tma_load_2d(b_dst, &tmB, full_bar(stage), k0, wgroup * args.N + nt * BN);
         }
         issued |= 1u << stage;
         issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
@@ -450,30 +472,84 @@ __global__ void __launch_bounds__(192, 1)
     const I8Rows rows = i8_rows(args, wgroup, row0);
     const float sx = row0 + lane < args.M ? __ldg(args.x_scale + row0 + lane) : 0.f;
     int sb = 0;
-    if (row0 < args.M) i8_stage_vectors(args, vecs, wgroup, rows, nt * (args.half > 0 ? BN / 2 : BN), lane);
+    const int width = args.half > 0 ? args.half : args.N;
+    const int per_tile = args.half > 0 ? BN / 2 : BN;
+    const int col0 = nt * per_tile;
+    if (row0 < args.M && splits == 1) i8_stage_vectors(args, vecs, wgroup, rows, col0, lane);
     if (row0 < args.M && mbar_wait(accf_bar, 0, abort_flag, args.status, kStatusTimeoutEpilogue)) {
       __syncwarp();
       tc_fence_after();
       const uint32_t tbase = tmem_base + (static_cast<uint32_t>(ew * 32) << 16);
-      const int width = args.half > 0 ? args.half : args.N;
-      const int per_tile = args.half > 0 ? BN / 2 : BN;
+      if (splits == 1) {
 #pragma unroll 1
-      for (int c = 0; c < per_tile / 32; ++c) {
-        const int ocol = nt * per_tile + c * 32;
-        if (ocol >= width) break;
-        uint32_t r[32], r2[32];
-        tmem_ld32(tbase + c * 32, r);
-        if (args.half > 0) tmem_ld32(tbase + BN / 2 + c * 32, r2);
-        tmem_ld_wait();
-        i8_chunk(args, &tmC, rows, row0, ocol, c * 32, sx, r, r2, vecs, buf, sb, lane);
+        for (int c = 0; c < per_tile / 32 && col0 + c * 32 < width; ++c) {
+          uint32_t r[32], r2[32];
+          tmem_ld32(tbase + c * 32, r);
+          if (args.half > 0) tmem_ld32(tbase + BN / 2 + c * 32, r2);
+          tmem_ld_wait();
+          i8_chunk(args, &tmC, rows, row0, col0 + c * 32, c * 32, sx, r, r2, vecs, buf, sb, lane);
+        }
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < BN / 32; ++c) {
+          uint32_t r[32];
+          tmem_ld32(tbase + c * 32, r);
+          tmem_ld_wait();
+          const uint32_t dst = sbase + (c * 32 * 128 + ew * 32 + lane) * 4;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + i * 512), "r"(r[i]) : "memory");
+        }
       }
       tc_fence_before();
     }
-    if (lane == 0) bulk_wait<0>();
-    __syncwarp();
+    if (splits == 1 && lane == 0) bulk_wait<0>();
   }
+  __syncwarp();
   tc_fence_before();
-  __syncthreads();
+  if (splits == 1) {
+    __syncthreads();
+  } else {
+    // Every CTA of the cluster gets here, timed out or not.
+    cluster_sync_all();
+    if (warp >= 2) {
+      const int ew = warp - 2;
+      const uint32_t buf = sbase + L::kEpiOffset + ew * 4096;
+      const uint32_t vecs = sbase + L::kVecOffset + ew * kI8VecWords * 4;
+      const int width = args.half > 0 ? args.half : args.N;
+      const int per_tile = args.half > 0 ? BN / 2 : BN;
+      const int col0 = nt * per_tile;
+      const int quarters = min(4, (args.M - m0 + 31) / 32);  // of rows that exist
+      const int chunks = min(per_tile / 32, (width - col0 + 31) / 32);
+      int sb = 0;
+      // Chunk u of the tile: its columns are u / quarters, its rows u % quarters.
+#pragma unroll 1
+      for (int u = rank + splits * ew; u < quarters * chunks; u += 4 * splits) {
+        const int c = u / quarters, q = u % quarters;
+        const int row0 = m0 + q * 32;
+        const I8Rows rows = i8_rows(args, wgroup, row0);
+        i8_stage_vectors(args, vecs, wgroup, rows, col0, lane);
+        const float sx = row0 + lane < args.M ? __ldg(args.x_scale + row0 + lane) : 0.f;
+        const uint32_t at = sbase + (c * 32 * 128 + q * 32 + lane) * 4;
+        uint32_t r[32], r2[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) r[i] = r2[i] = 0u;
+#pragma unroll 1
+        for (int s = 0; s < splits; ++s) {
+          const uint32_t src = mapa_shared(at, static_cast<uint32_t>(s));
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] += ld_shared_cluster(src + i * 512);
+          if (args.half > 0) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r2[i] += ld_shared_cluster(src + BN / 2 * 512 + i * 512);
+          }
+        }
+        i8_chunk(args, &tmC, rows, row0, col0 + c * 32, c * 32, sx, r, r2, vecs, buf, sb, lane);
+      }
+      if (lane == 0) bulk_wait<0>();
+      __syncwarp();
+    }
+    cluster_sync_all();  // no shared memory goes away while a peer reads it
+  }
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem_base, BN);
 }

@@ -9,6 +9,7 @@ These mirror the operator checks of the reference's smoke command
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -229,33 +230,71 @@ def modulate(x: torch.Tensor, shift: torch.Tensor | None, scale: torch.Tensor, *
     return out
 
 
-def _ld(t: torch.Tensor, multiple: int = 1) -> int:
-    """The row stride of a matrix; a single row's is never used and may be anything."""
-    return t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // multiple) * multiple
+# The wrappers from here to linear_w8a8 run before kernels of a few
+# microseconds, so they read each tensor attribute once and pack the C struct
+# in one call (filling a ctypes Structure takes four times as long).
+def _packer(args):
+    """struct's pack for a ctypes Structure's fields, in their native layout."""
+    fmt = struct.Struct("@" + "".join({C.c_int: "i", C.c_int64: "q", C.c_float: "f", C.c_void_p: "P"}[t]
+                                      for _, t in args._fields_))
+    pad = C.sizeof(args) - fmt.size
+    return fmt.pack if pad == 0 else lambda *values: fmt.pack(*values) + bytes(pad)
 
 
-def _padded(rows: int, cols: int, multiple: int, device, dtype) -> torch.Tensor:
-    """An uninitialised [rows, cols] matrix whose row stride is a multiple of `multiple`."""
-    wide = -(-cols // multiple) * multiple
+_pack_residual_norm, _pack_linear_w8a8 = _packer(ResidualNormArgs), _packer(LinearW8A8Args)
+
+
+def _addr(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _round_up(n: int, multiple: int) -> int:
+    return (n + multiple - 1) // multiple * multiple
+
+
+def _matrix(what: str, t: torch.Tensor, dtypes, device, multiple: int = 1) -> tuple[int, int, int]:
+    """Rows, columns and row stride of a matrix with unit column stride. A single row's stride is never used and may
+    be anything: the next multiple of `multiple` then."""
+    if t.dtype in dtypes and t.device == device:
+        shape, stride = t.shape, t.stride()
+        if len(shape) == 2:
+            rows, cols = shape
+            if stride[1] == 1 or cols == 1:
+                return rows, cols, stride[0] if rows > 1 else _round_up(cols, multiple)
+    raise ValueError(f"{what} must be a 2-D {'/'.join(str(d) for d in dtypes)} tensor with unit column stride on "
+                     f"{device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+
+
+def _output(what: str, t: torch.Tensor, rows: int, cols: int, dtypes, device, multiple: int = 1) -> int:
+    """The row stride of a caller's output, which must hold [rows, cols]."""
+    have, wide, ld = _matrix(what, t, dtypes, device, multiple)
+    if have < rows or wide < cols:
+        raise ValueError(f"{what} must be at least [{rows}, {cols}], got {tuple(t.shape)}")
+    return ld
+
+
+def _padded(rows: int, cols: int, multiple: int, device, dtype) -> tuple[torch.Tensor, int]:
+    """An uninitialised [rows, cols] matrix whose row stride is a multiple of `multiple`, and that stride."""
+    wide = _round_up(cols, multiple)
     t = torch.empty(rows, wide, device=device, dtype=dtype)
-    return t if wide == cols else t[:, :cols]
-
-
-def _check_matrix(what: str, t: torch.Tensor, dtypes, device) -> None:
-    if t.dim() != 2 or t.dtype not in dtypes or t.device != device or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"{what} must be a 2-D {'/'.join(str(d) for d in dtypes)} tensor with unit column stride on "
-                         f"{device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    return (t if wide == cols else t[:, :cols]), wide
 
 
 def _launch(what: str, device, fn, *args) -> None:
     """Call an op on the current stream of the tensors' device."""
     if device.type != "cuda":
         raise ValueError(f"{what}: the tensors must be on a CUDA device, got {device}")
+    stream = torch._C._cuda_getCurrentRawStream(device.index)  # what current_stream(device).cuda_stream reads
     if device.index == torch.cuda.current_device():
-        check(fn(*args, C.c_void_p(torch.cuda.current_stream(device).cuda_stream)))
-        return
-    with torch.cuda.device(device):
-        check(fn(*args, C.c_void_p(torch.cuda.current_stream(device).cuda_stream)))
+        code = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            code = fn(*args, stream)
+    if code:
+        check(code)
+
+
+_FP32, _INT8, _HALVES = (torch.float32,), (torch.int8,), (torch.bfloat16, torch.float16)
 
 
 def residual_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *, x_out: torch.Tensor | None = None,
@@ -275,41 +314,47 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *, x_out:
     vecs - 1). out_dtype None: x' only; torch.int8: one scale per row.
     Returns (x', y), (x', q, y_scale) for int8, or (x', None).
     """
-    _check_matrix("residual_norm: x", x, (torch.float32,), x.device)
-    rows, width = x.shape
     device = x.device
+    rows, width, ldx = _matrix("residual_norm: x", x, _FP32, device)
+    ldb = b_type = ldo = 0
     if branch is not None:
-        _check_matrix("residual_norm: branch", branch, _FLOATS, device)
-        if tuple(branch.shape) != (rows, width):
+        have, wide, ldb = _matrix("residual_norm: branch", branch, _FLOATS, device)
+        if have != rows or wide != width:
             raise ValueError(f"residual_norm: branch must be [{rows}, {width}], got {tuple(branch.shape)}")
-    _check_vec("residual_norm: post_weight", post_weight, width, device)
-    _check_vec("residual_norm: pre_weight", pre_weight, width, device)
-    vecs, stride = 1, width
-    sets = [(n, t) for n, t in (("gate", gate), ("scale", scale), ("shift", shift)) if t is not None]
-    if sets:
-        first = sets[0][1]
-        vecs = 1 if first.dim() == 1 else first.shape[0]
-        stride = first.stride(0) if vecs > 1 else width
-        for name, t in sets:
-            if (t.dim() not in (1, 2) or t.shape[-1] != width or (width > 1 and t.stride(-1) != 1)
-                    or t.dtype != torch.float32 or t.device != device or (1 if t.dim() == 1 else t.shape[0]) != vecs
-                    or (vecs > 1 and t.stride(0) != stride)):
-                raise ValueError(f"residual_norm: {name} must be float32 [{width}] or [vecs, {width}] on {device}, with "
-                                 f"the others' number of sets and row stride, got {tuple(t.shape)} {t.dtype}")
+        b_type = _DT[branch.dtype]
+    if post_weight is not None:
+        _check_vec("residual_norm: post_weight", post_weight, width, device)
+    if pre_weight is not None:
+        _check_vec("residual_norm: pre_weight", pre_weight, width, device)
+    vecs, vec_stride = 0, width
+    for name, t in (("gate", gate), ("scale", scale), ("shift", shift)):
+        if t is None:
+            continue
+        if t.dim() == 1:
+            t = t[None]
+        sets, wide, stride = _matrix(f"residual_norm: {name}", t, _FP32, device)
+        if vecs == 0:
+            vecs, vec_stride = sets, stride
+        if wide != width or sets != vecs or stride != vec_stride:
+            raise ValueError(f"residual_norm: {name} must be [{width}] or [vecs, {width}] with the others' number of "
+                             f"sets and row stride, got {tuple(t.shape)} with stride {stride}")
     if vecs > 1 and rows_per_vec <= 0:
         raise ValueError("residual_norm: several vector sets need rows_per_vec")
+    x_new = x
     if x_out is not None:
-        _check_out("residual_norm: x_out", x_out, rows, width, (torch.float32,), device)
+        ldo = _output("residual_norm: x_out", x_out, rows, width, _FP32, device)
+        x_new = x_out
     elif branch is not None or residual_scale != 1.0:
-        x_out = x
+        x_out, ldo = x, ldx
+    ldy = y_type = 0
     if out is not None:
-        _check_out("residual_norm: out", out, rows, width, (*_FLOATS, torch.int8), device)
+        ldy = _output("residual_norm: out", out, rows, width, (*_FLOATS, torch.int8), device)
         out_dtype = out.dtype
     elif out_dtype is not None:
         if out_dtype not in _DT8:
             raise ValueError(f"residual_norm: out_dtype must be a float type, torch.int8 or None, got {out_dtype}")
-        out = _padded(rows, width, 16 if out_dtype == torch.int8 else 1, device, out_dtype)
-    int8 = out_dtype == torch.int8
+        out, ldy = _padded(rows, width, 16 if out_dtype is torch.int8 else 1, device, out_dtype)
+    int8 = out_dtype is torch.int8
     if int8:
         if out_scale is None:
             out_scale = torch.empty(rows, device=device, dtype=torch.float32)
@@ -317,14 +362,13 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *, x_out:
             _check_vec("residual_norm: out_scale", out_scale, rows, device)
     elif out_scale is not None:
         raise ValueError("residual_norm: out_scale goes with an int8 output")
-    a = ResidualNormArgs(rows, width, x.data_ptr(), _ld(x), _ptr(x_out), _ld(x_out) if x_out is not None else 0,
-                         _ptr(branch), _ld(branch) if branch is not None else 0,
-                         _DT[branch.dtype] if branch is not None else 0, post_norm, _ptr(post_weight), _ptr(gate),
-                         residual_scale, pre_norm, _ptr(pre_weight), _ptr(scale), _ptr(shift), vecs, stride,
-                         rows_per_vec, int(plus_one), eps, _ptr(out), _ld(out) if out is not None else 0,
-                         _DT8[out_dtype] if out is not None else 0, _ptr(out_scale))
-    _launch("residual_norm", device, lib().nd_op_residual_norm, C.byref(a))
-    x_new = x if x_out is None else x_out
+    if out is not None:
+        y_type = _DT8[out_dtype]
+    a = _pack_residual_norm(rows, width, x.data_ptr(), ldx, _addr(x_out), ldo, _addr(branch), ldb, b_type, post_norm,
+                            _addr(post_weight), _addr(gate), residual_scale, pre_norm, _addr(pre_weight), _addr(scale),
+                            _addr(shift), vecs or 1, vec_stride, rows_per_vec, 1 if plus_one else 0, eps, _addr(out), ldy,
+                            y_type, _addr(out_scale))
+    _launch("residual_norm", device, lib().nd_op_residual_norm, a)
     return (x_new, out, out_scale) if int8 else (x_new, out)
 
 
@@ -333,18 +377,18 @@ def quantize_rows(x: torch.Tensor, *, out: torch.Tensor | None = None,
     """Rows (tokens) as int8 with one scale each: scale = max |x| / 127 over the row, q = rint(x * 127 / max |x|),
     the quotient rounded as if exact. Returns (q [rows, cols], scale [rows]); q's rows are a multiple of 16 bytes
     apart, as linear_w8a8 reads them. A row with an infinity or a NaN gets scale NaN and q 0."""
-    _check_matrix("quantize_rows: x", x, _FLOATS, x.device)
-    rows, cols = x.shape
+    device = x.device
+    rows, cols, ldx = _matrix("quantize_rows: x", x, _FLOATS, device)
     if out is None:
-        out = _padded(rows, cols, 16, x.device, torch.int8)
+        out, ldq = _padded(rows, cols, 16, device, torch.int8)
     else:
-        _check_out("quantize_rows: out", out, rows, cols, (torch.int8,), x.device)
+        ldq = _output("quantize_rows: out", out, rows, cols, _INT8, device, 16)
     if scale is None:
-        scale = torch.empty(rows, device=x.device, dtype=torch.float32)
+        scale = torch.empty(rows, device=device, dtype=torch.float32)
     else:
-        _check_vec("quantize_rows: scale", scale, rows, x.device)
-    _launch("quantize_rows", x.device, lib().nd_op_quantize_rows, x.data_ptr(), _DT[x.dtype], rows, cols, _ld(x),
-            out.data_ptr(), _ld(out), scale.data_ptr())
+        _check_vec("quantize_rows: scale", scale, rows, device)
+    _launch("quantize_rows", device, lib().nd_op_quantize_rows, x.data_ptr(), _DT[x.dtype], rows, cols, ldx,
+            out.data_ptr(), ldq, scale.data_ptr())
     return out, scale
 
 
@@ -364,44 +408,46 @@ def linear_w8a8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, w_
     one if none is given. SWIGLU / GEGLU: weight [2F, in], output [rows, F].
     """
     device = x.device
-    _check_matrix("linear_w8a8: x", x, (torch.int8,), device)
-    _check_matrix("linear_w8a8: weight", weight, (torch.int8,), device)
-    rows, k = x.shape
+    rows, k, ldx = _matrix("linear_w8a8: x", x, _INT8, device, 16)
+    w_rows, w_cols, ldw = _matrix("linear_w8a8: weight", weight, _INT8, device, 16)
     split = group_split is not None and group_split < rows
     groups = 2 if split and not shared_weights else 1
     gated = epilogue in (_lib.ND_EPI_SWIGLU, _lib.ND_EPI_GEGLU)
-    each = weight.shape[0] // groups
+    each = w_rows // groups
     n = each // 2 if gated else each
-    if weight.shape[1] != k or each * groups != weight.shape[0] or (gated and each % 2):
+    if w_cols != k or each * groups != w_rows or (gated and each % 2):
         raise ValueError(f"linear_w8a8: weight must be [{groups} * {'2 * ' if gated else ''}out, {k}], got {tuple(weight.shape)}")
     _check_vec("linear_w8a8: x_scale", x_scale, rows, device)
-    _check_vec("linear_w8a8: w_scale", w_scale, weight.shape[0], device)
-    _check_vec("linear_w8a8: bias", bias, (2 if split else 1) * each, device)
-    _check_vec("linear_w8a8: gate", gate, (2 if split else 1) * n, device)
+    _check_vec("linear_w8a8: w_scale", w_scale, w_rows, device)
+    if bias is not None:
+        _check_vec("linear_w8a8: bias", bias, (2 if split else 1) * each, device)
+    if gate is not None:
+        _check_vec("linear_w8a8: gate", gate, (2 if split else 1) * n, device)
+    ldy = ldr = lda = 0
     if epilogue in (_lib.ND_EPI_RESIDUAL_GATE, _lib.ND_EPI_RESIDUAL_ADD, _lib.ND_EPI_STORE_F32):
         if residual is not None:
-            _check_out("linear_w8a8: residual", residual, rows, n, (torch.float32,), device)
+            ldr = _output("linear_w8a8: residual", residual, rows, n, _FP32, device, 4)
         elif epilogue == _lib.ND_EPI_STORE_F32:
-            residual = _padded(rows, n, 4, device, torch.float32)
+            residual, ldr = _padded(rows, n, 4, device, torch.float32)
         else:
             raise ValueError("linear_w8a8: this epilogue adds to residual, and none is given")
         out, out_dtype = None, torch.bfloat16
-    elif out is not None:
-        _check_out("linear_w8a8: out", out, rows, n, (torch.float16, torch.bfloat16), device)
-        out_dtype, residual = out.dtype, None
     else:
-        if out_dtype not in (torch.float16, torch.bfloat16):
+        residual = None
+        if out is not None:
+            ldy = _output("linear_w8a8: out", out, rows, n, _HALVES, device, 8)
+            out_dtype = out.dtype
+        elif out_dtype in _HALVES:
+            out, ldy = _padded(rows, n, 8, device, out_dtype)
+        else:
             raise ValueError(f"linear_w8a8: out_dtype must be float16 or bfloat16 (STORE_F32 for fp32), got {out_dtype}")
-        out, residual = _padded(rows, n, 8, device, out_dtype), None
     if addend is not None:
-        _check_out("linear_w8a8: addend", addend, rows, n, (out_dtype,), device)
-    a = LinearW8A8Args(_DT[out_dtype], epilogue, rows, k, n, x.data_ptr(), _ld(x, 16), x_scale.data_ptr(),
-                       weight.data_ptr(), _ld(weight, 16), w_scale.data_ptr(), _ptr(bias),
-                       group_split if group_split is not None else rows, int(shared_weights),
-                       _ptr(out), _ld(out, 8) if out is not None else 0,
-                       _ptr(residual), _ld(residual, 4) if residual is not None else 0,
-                       _ptr(gate), 0, _ptr(addend), _ld(addend, 8) if addend is not None else 0)
-    _launch("linear_w8a8", device, lib().nd_op_linear_w8a8, C.byref(a))
+        lda = _output("linear_w8a8: addend", addend, rows, n, (out_dtype,), device)
+    a = _pack_linear_w8a8(_DT[out_dtype], epilogue, rows, k, n, x.data_ptr(), ldx, x_scale.data_ptr(), weight.data_ptr(),
+                          ldw, w_scale.data_ptr(), _addr(bias), rows if group_split is None else group_split,
+                          1 if shared_weights else 0, _addr(out), ldy, _addr(residual), ldr, _addr(gate), 0,
+                          _addr(addend), lda)
+    _launch("linear_w8a8", device, lib().nd_op_linear_w8a8, a)
     return out if residual is None else residual
 
 
