@@ -3,11 +3,12 @@
 //
 //   scale[r] = max |x[r]| / 127,   q[r, c] = rint(x[r, c] * 127 / max |x[r]|)
 //
-// The quotient is rounded as if computed exactly, half to even: the fast
-// product x * (127 / peak) is at most 2^-23 * 127 off, so only values whose
-// product lies within that of a half are divided again, in double, where
-// x * 127 is exact and no quotient of two fp32 values lies closer to a half
-// than a double resolves without being one.
+// The quotient is rounded as if computed exactly, half to even. The fast
+// product t = x * (127 / peak) is off by at most 2^-23 * 127; only where t lies
+// that near a half is its integer r checked against x * 127 - r * peak, which
+// two products and their fma remainders give exactly (near_half below). A
+// second pass over the thread's values with double division instead took 99 us
+// at 4352 x 12288: values of exactly half the peak make one in most rows.
 //
 // Bound by HBM: the row is read once, stays in registers while its peak is
 // found, and one byte per value is written.
@@ -26,28 +27,28 @@ namespace {
 // The fast product x * (127 / peak) is off by at most 2^-23 * 127 = 1.5e-5.
 constexpr float kNearHalf = 0.49997f;
 
-// VEC values of type ND_F32 / ND_F16 / ND_BF16 as fp32.
+// VEC values of type ND_F32 / ND_F16 / ND_BF16 as fp32: VEC 8 or 1.
 template <int VEC>
 __device__ __forceinline__ void load_vals(const void* p, long long i, int type, float (&f)[VEC]) {
-  if constexpr (VEC == 4) {
+  if constexpr (VEC == 8) {
+    uint32_t w[4];
     if (type == ND_F32) {
-      asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0,%1,%2,%3}, [%4];"
-                   : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3])
-                   : "l"(static_cast<const float*>(p) + i));
-    } else {
-      uint32_t a, b;
-      asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];"
-                   : "=r"(a), "=r"(b)
-                   : "l"(static_cast<const uint16_t*>(p) + i));
-      float2 lo, hi;
-      if (type == ND_F16) {
-        lo = __half22float2(*reinterpret_cast<const __half2*>(&a));
-        hi = __half22float2(*reinterpret_cast<const __half2*>(&b));
-      } else {
-        lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&a));
-        hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&b));
-      }
-      f[0] = lo.x; f[1] = lo.y; f[2] = hi.x; f[3] = hi.y;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0,%1,%2,%3}, [%4];"
+                     : "=f"(f[4 * h]), "=f"(f[4 * h + 1]), "=f"(f[4 * h + 2]), "=f"(f[4 * h + 3])
+                     : "l"(static_cast<const float*>(p) + i + 4 * h));
+      return;
+    }
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "l"(static_cast<const uint16_t*>(p) + i));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 t = type == ND_F16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[j]))
+                                      : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[j]));
+      f[2 * j] = t.x;
+      f[2 * j + 1] = t.y;
     }
   } else {
     f[0] = type == ND_F32   ? __ldg(static_cast<const float*>(p) + i)
@@ -56,52 +57,71 @@ __device__ __forceinline__ void load_vals(const void* p, long long i, int type, 
   }
 }
 
-// The exact quotient's nearest integer, as bits whose low byte is q.
-__device__ __forceinline__ uint32_t rint_exact(float x, float peak) {
-  return static_cast<uint32_t>(__double2int_rn(__ddiv_rn(static_cast<double>(x) * 127.0, static_cast<double>(peak))));
+// The exact rounding of x * 127 / peak, given r, its integer by the fast
+// product, where the quotient lies near r +- 1/2. 127 x = hi + lo and
+// r peak = hi2 + lo2 exactly (fma remainders); hi - hi2, 2 |d| - peak and
+// lo - lo2 are differences of near neighbours or of few bits and exact, so the
+// sign of their sum says on which side of the half the quotient lies.
+__device__ __forceinline__ float near_half(float x, float r, float peak) {
+  const float hi = x * 127.0f, lo = fmaf(x, 127.0f, -hi);
+  const float hi2 = r * peak, lo2 = fmaf(r, peak, -hi2);
+  const float d = hi - hi2;
+  const float way = d < 0.f ? -1.f : 1.f;
+  const float past = (2.f * fabsf(d) - peak) + 2.f * way * (lo - lo2);
+  const bool odd = (__float2int_rn(r) & 1) != 0;
+  return past > 0.f || (past == 0.f && odd) ? r + way : r;
 }
 
-// VEC values by the fast product; returns their largest distance from the
-// integer taken.
+// VEC values (already multiplied by `shift`'s power of two) to int8.
 template <int VEC>
-__device__ __forceinline__ float quantize_store(int8_t* q, const float (&f)[VEC], float inverse) {
-  uint32_t u[4] = {0u, 0u, 0u, 0u};
+__device__ __forceinline__ void quantize_store(int8_t* q, const float (&f)[VEC], float inverse, float peak) {
+  float m[VEC];  // rint(t) + 1.5 * 2^23
   float most = 0.f;
 #pragma unroll
   for (int j = 0; j < VEC; ++j) {
-    float off;
-    u[j] = rint_bits(f[j] * inverse, off);
-    most = fmaxf(most, off);
+    const float t = f[j] * inverse;
+    m[j] = t + kRintMagic;
+    most = fmaxf(most, fabsf(t - (m[j] - kRintMagic)));
   }
-  if constexpr (VEC == 4) *reinterpret_cast<uint32_t*>(q) = pack_low_bytes(u[0], u[1], u[2], u[3]);
-  else *q = static_cast<int8_t>(u[0] & 0xffu);
-  return most;
+  if (most > kNearHalf) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) m[j] = near_half(f[j], m[j] - kRintMagic, peak) + kRintMagic;
+  }
+  if constexpr (VEC == 8) {
+    *reinterpret_cast<uint2*>(q) =
+        make_uint2(pack_low_bytes(__float_as_uint(m[0]), __float_as_uint(m[1]), __float_as_uint(m[2]), __float_as_uint(m[3])),
+                   pack_low_bytes(__float_as_uint(m[4]), __float_as_uint(m[5]), __float_as_uint(m[6]), __float_as_uint(m[7])));
+  } else {
+    *q = static_cast<int8_t>(__float_as_uint(m[0]) & 0xffu);
+  }
 }
 
+template <int T>
 __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
   v = __reduce_max_sync(0xffffffffu, v);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
   v = red[0];
-  for (int i = 1; i < static_cast<int>(blockDim.x >> 5); ++i) v = max(v, red[i]);
+#pragma unroll
+  for (int i = 1; i < T / 32; ++i) v = max(v, red[i]);
   return v;
 }
 
 // One block per row; V x VEC values per thread in registers, the rest of a
 // longer row read twice.
-template <int VEC, int V>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const void* x, long long ldx, int type, int width,
+template <int VEC, int V, int T>
+__global__ void __launch_bounds__(T) quantize_rows_kernel(const void* x, long long ldx, int type, int width,
                                                             int8_t* q, long long ldq, float* scale) {
   griddep_launch();
   griddep_wait();
-  __shared__ uint32_t red[8];
+  __shared__ uint32_t red[T / 32];
   const long long r = blockIdx.x;
   const long long x0 = r * ldx;
   float v[V][VEC];
   uint32_t peak = 0u;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int c = (threadIdx.x + blockDim.x * i) * VEC;
+    const int c = (threadIdx.x + T * i) * VEC;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) v[i][j] = 0.f;
     if (c < width) load_vals<VEC>(x, x0 + c, type, v[i]);
@@ -110,48 +130,42 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* x, long 
   for (int i = 0; i < V; ++i)
 #pragma unroll
     for (int j = 0; j < VEC; ++j) peak = max(peak, abs_bits(v[i][j]));
-  for (int c = (threadIdx.x + blockDim.x * V) * VEC; c < width; c += blockDim.x * VEC) {
+  for (int c = (threadIdx.x + T * V) * VEC; c < width; c += T * VEC) {
     float w[VEC];
     load_vals<VEC>(x, x0 + c, type, w);
 #pragma unroll
     for (int j = 0; j < VEC; ++j) peak = max(peak, abs_bits(w[j]));
   }
-  const RowScale s = row_scale(block_max(peak, red));
+  const RowScale s = row_scale(block_max<T>(peak, red));
   if (threadIdx.x == 0) scale[r] = s.scale;
   int8_t* out = q + r * ldq;
   if (s.inverse == 0.f) {  // zeros, or infinities and NaN: every q is 0
     const float zero[VEC] = {};
 #pragma unroll 1
-    for (int c = threadIdx.x * VEC; c < width; c += blockDim.x * VEC) quantize_store<VEC>(out + c, zero, 0.f);
+    for (int c = threadIdx.x * VEC; c < width; c += T * VEC) quantize_store<VEC>(out + c, zero, 0.f, 1.f);
     return;
   }
-  float most = 0.f;
+  // Where 127 / peak or 127 x would leave fp32's range, the row is worked on
+  // times a power of two (which changes no quotient).
+  const float shift = s.peak < 1e-30f ? 0x1p96f : s.peak > 1e30f ? 0x1p-64f : 1.f;
+  const float row_peak = s.peak * shift;
+  const float inverse = shift == 1.f ? s.inverse : __fdiv_rn(127.0f, row_peak);
+  auto finish = [&](int c, float(&w)[VEC]) {
+    if (shift != 1.f) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) w[j] *= shift;
+    }
+    quantize_store<VEC>(out + c, w, inverse, row_peak);
+  };
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int c = (threadIdx.x + blockDim.x * i) * VEC;
-    if (c < width) most = fmaxf(most, quantize_store<VEC>(out + c, v[i], s.inverse));
+    const int c = (threadIdx.x + T * i) * VEC;
+    if (c < width) finish(c, v[i]);
   }
-  for (int c = (threadIdx.x + blockDim.x * V) * VEC; c < width; c += blockDim.x * VEC) {
+  for (int c = (threadIdx.x + T * V) * VEC; c < width; c += T * VEC) {
     float w[VEC];
     load_vals<VEC>(x, x0 + c, type, w);
-    most = fmaxf(most, quantize_store<VEC>(out + c, w, s.inverse));
-  }
-  // Rare (one thread in a few hundred): a value whose quotient may lie on the
-  // other side of a half, or a row whose 127 / peak leaves fp32's range. The
-  // thread's values are read again, out of the cache, and those divided.
-  const bool tiny = s.peak < 1e-30f;
-  if (tiny || most > kNearHalf) {
-#pragma unroll 1
-    for (int c = threadIdx.x * VEC; c < width; c += blockDim.x * VEC) {
-      float w[VEC];
-      load_vals<VEC>(x, x0 + c, type, w);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        float off;
-        rint_bits(w[j] * s.inverse, off);
-        if (tiny || off > kNearHalf) out[c + j] = static_cast<int8_t>(rint_exact(w[j], s.peak) & 0xffu);
-      }
-    }
+    finish(c, w);
   }
 }
 
@@ -165,22 +179,23 @@ int quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t 
   if (rows > INT_MAX || cols > INT_MAX / 2) return fail(ND_ERR_INVALID, "quantize_rows: shape too large");
   if (!x || !q || !scale) return fail(ND_ERR_INVALID, "quantize_rows: null operand");
   if (ldx < cols || ldq < cols) return fail(ND_ERR_INVALID, "quantize_rows: a row stride is smaller than cols");
-  const int elem = dtype == ND_F32 ? 4 : 2;
-  const bool by4 = cols % 4 == 0 && ldx % 4 == 0 && ldq % 4 == 0 && reinterpret_cast<uintptr_t>(x) % (4 * elem) == 0 &&
-                   reinterpret_cast<uintptr_t>(q) % 4 == 0;
+  const bool by8 = cols % 8 == 0 && ldx % 8 == 0 && ldq % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(q) % 8 == 0;
   const dim3 grid(static_cast<unsigned>(rows));
   const int w = static_cast<int>(cols);
 #define ND_QR(VEC, V, T) \
-  ND_CUDA(launch_pdl(quantize_rows_kernel<VEC, V>, grid, dim3(T), 0, stream, x, ldx, dtype, w, q, ldq, scale))
-  if (by4) {
-    const int64_t w4 = cols / 4;
-    if (w4 <= 128) ND_QR(4, 1, 128);
-    else if (w4 <= 512) ND_QR(4, 4, 128);
-    else if (w4 <= 1024) ND_QR(4, 4, 256);
-    else ND_QR(4, 12, 256);
+  ND_CUDA(launch_pdl(quantize_rows_kernel<VEC, V, T>, grid, dim3(T), 0, stream, x, ldx, dtype, w, q, ldq, scale))
+  if (by8) {
+    const int64_t w8 = cols / 8;
+    if (w8 <= 128) ND_QR(8, 1, 128);
+    else if (w8 <= 256) ND_QR(8, 2, 128);
+    else if (w8 <= 512) ND_QR(8, 2, 256);
+    else if (w8 <= 1024) ND_QR(8, 2, 512);
+    else ND_QR(8, 3, 512);
   } else {
-    if (cols <= 512) ND_QR(1, 4, 128);
-    else ND_QR(1, 24, 256);
+    if (cols <= 1024) ND_QR(1, 4, 256);
+    else if (cols <= 4096) ND_QR(1, 16, 256);
+    else ND_QR(1, 16, 512);
   }
 #undef ND_QR
   ND_CUDA(cudaGetLastError());

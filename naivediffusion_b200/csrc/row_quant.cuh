@@ -35,14 +35,9 @@ __device__ __forceinline__ RowScale row_scale(uint32_t peak_bits) {
   return r;
 }
 
-// rint(t) for |t| < 2^22 as an integer in the low bits of the result (adding
-// 1.5 * 2^23 leaves no fraction bits; round to nearest even), and t's
-// distance from it.
-__device__ __forceinline__ uint32_t rint_bits(float t, float& off) {
-  const float m = t + 12582912.0f;
-  off = fabsf(t - (m - 12582912.0f));
-  return __float_as_uint(m);
-}
+// t + kRintMagic (1.5 * 2^23) leaves no fraction bits: for |t| < 2^22 its low
+// bits are rint(t), round to nearest even.
+constexpr float kRintMagic = 12582912.0f;
 
 // Four values' low bytes as one word.
 __device__ __forceinline__ uint32_t pack_low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -51,8 +46,8 @@ __device__ __forceinline__ uint32_t pack_low_bytes(uint32_t a, uint32_t b, uint3
 
 // Four values, already scaled to [-127, 127].
 __device__ __forceinline__ uint32_t pack_rint(float a, float b, float c, float d) {
-  float off;
-  return pack_low_bytes(rint_bits(a, off), rint_bits(b, off), rint_bits(c, off), rint_bits(d, off));
+  return pack_low_bytes(__float_as_uint(a + kRintMagic), __float_as_uint(b + kRintMagic), __float_as_uint(c + kRintMagic),
+                        __float_as_uint(d + kRintMagic));
 }
 
 }  // namespace nd
