@@ -27,34 +27,84 @@ namespace {
 // The fast product x * (127 / peak) is off by at most 2^-23 * 127 = 1.5e-5.
 constexpr float kNearHalf = 0.49997f;
 
-// VEC values of type ND_F32 / ND_F16 / ND_BF16 as fp32: VEC 8 or 1.
-template <int VEC>
-__device__ __forceinline__ void load_vals(const void* p, long long i, int type, float (&f)[VEC]) {
-  if constexpr (VEC == 8) {
-    uint32_t w[4];
-    if (type == ND_F32) {
+// A thread's share of a row as it lies in memory: VEC values of one type. The
+// 16-bit types stay packed until they are quantized (half the registers, so
+// twice the rows in flight), and |x| is compared as integers: bit patterns of
+// one sign order like the values, with NaN above infinity.
+template <int TYPE, int VEC>
+struct Raw;
+template <>
+struct Raw<ND_F32, 8> {
+  float4 w[2];
+  __device__ __forceinline__ void clear() { w[0] = w[1] = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void load(const void* p, long long i) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0,%1,%2,%3}, [%4];"
-                     : "=f"(f[4 * h]), "=f"(f[4 * h + 1]), "=f"(f[4 * h + 2]), "=f"(f[4 * h + 3])
-                     : "l"(static_cast<const float*>(p) + i + 4 * h));
-      return;
+    for (int h = 0; h < 2; ++h)
+      asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0,%1,%2,%3}, [%4];"
+                   : "=f"(w[h].x), "=f"(w[h].y), "=f"(w[h].z), "=f"(w[h].w)
+                   : "l"(static_cast<const float*>(p) + i + 4 * h));
+  }
+  __device__ __forceinline__ void peak(uint32_t& m) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      m = max(max(m, max(abs_bits(w[h].x), abs_bits(w[h].y))), max(abs_bits(w[h].z), abs_bits(w[h].w)));
+  }
+  __device__ __forceinline__ void values(float (&f)[8]) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      f[4 * h] = w[h].x; f[4 * h + 1] = w[h].y; f[4 * h + 2] = w[h].z; f[4 * h + 3] = w[h].w;
     }
+  }
+};
+template <>
+struct Raw<ND_F32, 1> {
+  float w;
+  __device__ __forceinline__ void clear() { w = 0.f; }
+  __device__ __forceinline__ void load(const void* p, long long i) { w = __ldg(static_cast<const float*>(p) + i); }
+  __device__ __forceinline__ void peak(uint32_t& m) const { m = max(m, abs_bits(w)); }
+  __device__ __forceinline__ void values(float (&f)[1]) const { f[0] = w; }
+};
+template <int TYPE>
+__device__ __forceinline__ float2 halves(uint32_t w) {
+  if constexpr (TYPE == ND_F16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <int TYPE>
+struct Raw<TYPE, 8> {
+  uint4 w;
+  __device__ __forceinline__ void clear() { w = make_uint4(0u, 0u, 0u, 0u); }
+  __device__ __forceinline__ void load(const void* p, long long i) {
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
                  : "l"(static_cast<const uint16_t*>(p) + i));
+  }
+  __device__ __forceinline__ void peak(uint32_t& m) const {  // two 16-bit maxima
+    constexpr uint32_t k = 0x7fff7fffu;
+    m = __vmaxu2(__vmaxu2(m, __vmaxu2(w.x & k, w.y & k)), __vmaxu2(w.z & k, w.w & k));
+  }
+  __device__ __forceinline__ void values(float (&f)[8]) const {
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float2 t = type == ND_F16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[j]))
-                                      : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[j]));
+      const float2 t = halves<TYPE>(v[j]);
       f[2 * j] = t.x;
       f[2 * j + 1] = t.y;
     }
-  } else {
-    f[0] = type == ND_F32   ? __ldg(static_cast<const float*>(p) + i)
-           : type == ND_F16 ? __half2float(static_cast<const __half*>(p)[i])
-                            : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
   }
+};
+template <int TYPE>
+struct Raw<TYPE, 1> {
+  uint16_t w;
+  __device__ __forceinline__ void clear() { w = 0; }
+  __device__ __forceinline__ void load(const void* p, long long i) { w = __ldg(static_cast<const uint16_t*>(p) + i); }
+  __device__ __forceinline__ void peak(uint32_t& m) const { m = max(m, static_cast<uint32_t>(w & 0x7fff)); }
+  __device__ __forceinline__ void values(float (&f)[1]) const { f[0] = halves<TYPE>(w).x; }
+};
+// The peak's bits as fp32's.
+template <int TYPE>
+__device__ __forceinline__ uint32_t peak_bits(uint32_t m) {
+  if constexpr (TYPE == ND_F32) return m;
+  else return __float_as_uint(halves<TYPE>(max(m & 0xffffu, m >> 16)).x);
 }
 
 // The exact rounding of x * 127 / peak, given r, its integer by the fast
@@ -77,11 +127,21 @@ template <int VEC>
 __device__ __forceinline__ void quantize_store(int8_t* q, const float (&f)[VEC], float inverse, float peak) {
   float m[VEC];  // rint(t) + 1.5 * 2^23
   float most = 0.f;
+  if constexpr (VEC == 8) {
+    const float2 inv2 = make_float2(inverse, inverse), magic2 = make_float2(kRintMagic, kRintMagic);
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) {
-    const float t = f[j] * inverse;
-    m[j] = t + kRintMagic;
-    most = fmaxf(most, fabsf(t - (m[j] - kRintMagic)));
+    for (int j = 0; j < 8; j += 2) {
+      const float2 x2 = make_float2(f[j], f[j + 1]);
+      const float2 m2 = ffma2(x2, inv2, magic2);
+      const float2 r2 = fadd2(magic2, make_float2(-m2.x, -m2.y));
+      const float2 off = ffma2(x2, inv2, r2);
+      m[j] = m2.x;
+      m[j + 1] = m2.y;
+      most = fmax3(most, fabsf(off.x), fabsf(off.y));
+    }
+  } else {
+    m[0] = fmaf(f[0], inverse, kRintMagic);
+    most = fabsf(fmaf(f[0], inverse, kRintMagic - m[0]));
   }
   if (most > kNearHalf) {
 #pragma unroll
@@ -99,50 +159,53 @@ __device__ __forceinline__ void quantize_store(int8_t* q, const float (&f)[VEC],
 template <int T>
 __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
   v = __reduce_max_sync(0xffffffffu, v);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[0];
+  if constexpr (T > 32) {
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = red[0];
 #pragma unroll
-  for (int i = 1; i < T / 32; ++i) v = max(v, red[i]);
+    for (int i = 1; i < T / 32; ++i) v = max(v, red[i]);
+  }
   return v;
 }
 
-// One block per row; V x VEC values per thread in registers, the rest of a
-// longer row read twice.
-template <int VEC, int V, int T>
-__global__ void __launch_bounds__(T) quantize_rows_kernel(const void* x, long long ldx, int type, int width,
-                                                            int8_t* q, long long ldq, float* scale) {
+// T threads per row (a warp for narrow rows, four rows to a block), V x VEC
+// values per thread in registers, the rest of a longer row read twice.
+// 1536 threads per SM (40 registers; fp32 vectors take 64) keep enough rows in
+// flight.
+template <int TYPE, int VEC, int V, int T>
+__global__ void __launch_bounds__(T < 128 ? 128 : T, (TYPE == ND_F32 && VEC == 8 ? 1024 : 1536) / (T < 128 ? 128 : T))
+    quantize_rows_kernel(const void* x, long long ldx, int rows, int width, int8_t* q, long long ldq, float* scale) {
   griddep_launch();
   griddep_wait();
   __shared__ uint32_t red[T / 32];
-  const long long r = blockIdx.x;
+  constexpr int kRows = T < 128 ? 128 / T : 1;
+  const int t = threadIdx.x % T;
+  const long long r = static_cast<long long>(blockIdx.x) * kRows + threadIdx.x / T;
+  if (r >= rows) return;  // whole warps: only T = 32 has several rows per block
   const long long x0 = r * ldx;
-  float v[V][VEC];
+  Raw<TYPE, VEC> v[V];
   uint32_t peak = 0u;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int c = (threadIdx.x + T * i) * VEC;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) v[i][j] = 0.f;
-    if (c < width) load_vals<VEC>(x, x0 + c, type, v[i]);
+    const int c = (t + T * i) * VEC;
+    v[i].clear();
+    if (c < width) v[i].load(x, x0 + c);
   }
 #pragma unroll
-  for (int i = 0; i < V; ++i)
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) peak = max(peak, abs_bits(v[i][j]));
-  for (int c = (threadIdx.x + T * V) * VEC; c < width; c += T * VEC) {
-    float w[VEC];
-    load_vals<VEC>(x, x0 + c, type, w);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) peak = max(peak, abs_bits(w[j]));
+  for (int i = 0; i < V; ++i) v[i].peak(peak);
+  for (int c = (t + T * V) * VEC; c < width; c += T * VEC) {
+    Raw<TYPE, VEC> w;
+    w.load(x, x0 + c);
+    w.peak(peak);
   }
-  const RowScale s = row_scale(block_max<T>(peak, red));
-  if (threadIdx.x == 0) scale[r] = s.scale;
+  const RowScale s = row_scale(block_max<T>(peak_bits<TYPE>(peak), red));
+  if (t == 0) scale[r] = s.scale;
   int8_t* out = q + r * ldq;
   if (s.inverse == 0.f) {  // zeros, or infinities and NaN: every q is 0
     const float zero[VEC] = {};
 #pragma unroll 1
-    for (int c = threadIdx.x * VEC; c < width; c += T * VEC) quantize_store<VEC>(out + c, zero, 0.f, 1.f);
+    for (int c = t * VEC; c < width; c += T * VEC) quantize_store<VEC>(out + c, zero, 0.f, 1.f);
     return;
   }
   // Where 127 / peak or 127 x would leave fp32's range, the row is worked on
@@ -150,7 +213,9 @@ __global__ void __launch_bounds__(T) quantize_rows_kernel(const void* x, long lo
   const float shift = s.peak < 1e-30f ? 0x1p96f : s.peak > 1e30f ? 0x1p-64f : 1.f;
   const float row_peak = s.peak * shift;
   const float inverse = shift == 1.f ? s.inverse : __fdiv_rn(127.0f, row_peak);
-  auto finish = [&](int c, float(&w)[VEC]) {
+  auto finish = [&](int c, const Raw<TYPE, VEC>& raw) {
+    float w[VEC];
+    raw.values(w);
     if (shift != 1.f) {
 #pragma unroll
       for (int j = 0; j < VEC; ++j) w[j] *= shift;
@@ -159,14 +224,43 @@ __global__ void __launch_bounds__(T) quantize_rows_kernel(const void* x, long lo
   };
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int c = (threadIdx.x + T * i) * VEC;
+    const int c = (t + T * i) * VEC;
     if (c < width) finish(c, v[i]);
   }
-  for (int c = (threadIdx.x + T * V) * VEC; c < width; c += T * VEC) {
-    float w[VEC];
-    load_vals<VEC>(x, x0 + c, type, w);
+  for (int c = (t + T * V) * VEC; c < width; c += T * VEC) {
+    Raw<TYPE, VEC> w;
+    w.load(x, x0 + c);
     finish(c, w);
   }
+}
+
+template <int TYPE>
+int launch(const void* x, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
+           cudaStream_t stream) {
+  const bool by8 = cols % 8 == 0 && ldx % 8 == 0 && ldq % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(q) % 8 == 0;
+  const int w = static_cast<int>(cols), n = static_cast<int>(rows);
+#define ND_QR(VEC, V, T)                                                                                            \
+  ND_CUDA(launch_pdl(quantize_rows_kernel<TYPE, VEC, V, T>, dim3((n + (T < 128 ? 128 / T : 1) - 1) /                  \
+                     (T < 128 ? 128 / T : 1)), dim3(T < 128 ? 128 : T), 0, stream, x, ldx, n, w, q, ldq, scale))
+  if (by8) {
+    const int64_t w8 = cols / 8;
+    if (w8 <= 64) ND_QR(8, 2, 32);
+    else if (w8 <= 128) ND_QR(8, 4, 32);
+    else if (w8 <= 256) ND_QR(8, 2, 128);
+    else if (w8 <= 512) ND_QR(8, 4, 128);
+    else if (w8 <= 1024) ND_QR(8, 4, 256);
+    else if (w8 <= 1536) ND_QR(8, 3, 512);
+    else ND_QR(8, 4, 512);
+  } else {
+    if (cols <= 256) ND_QR(1, 8, 32);
+    else if (cols <= 2048) ND_QR(1, 8, 256);
+    else if (cols <= 4096) ND_QR(1, 8, 512);
+    else ND_QR(1, 12, 512);
+  }
+#undef ND_QR
+  ND_CUDA(cudaGetLastError());
+  return ND_OK;
 }
 
 }  // namespace
@@ -176,30 +270,12 @@ int quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t 
   if (dtype != ND_F32 && dtype != ND_F16 && dtype != ND_BF16)
     return fail(ND_ERR_INVALID, "quantize_rows: x must be f32, f16 or bf16");
   if (rows <= 0 || cols <= 0) return fail(ND_ERR_INVALID, "quantize_rows: empty shape");
-  if (rows > INT_MAX || cols > INT_MAX / 2) return fail(ND_ERR_INVALID, "quantize_rows: shape too large");
+  if (rows > INT_MAX - 128 || cols > INT_MAX / 2) return fail(ND_ERR_INVALID, "quantize_rows: shape too large");
   if (!x || !q || !scale) return fail(ND_ERR_INVALID, "quantize_rows: null operand");
   if (ldx < cols || ldq < cols) return fail(ND_ERR_INVALID, "quantize_rows: a row stride is smaller than cols");
-  const bool by8 = cols % 8 == 0 && ldx % 8 == 0 && ldq % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
-                   reinterpret_cast<uintptr_t>(q) % 8 == 0;
-  const dim3 grid(static_cast<unsigned>(rows));
-  const int w = static_cast<int>(cols);
-#define ND_QR(VEC, V, T) \
-  ND_CUDA(launch_pdl(quantize_rows_kernel<VEC, V, T>, grid, dim3(T), 0, stream, x, ldx, dtype, w, q, ldq, scale))
-  if (by8) {
-    const int64_t w8 = cols / 8;
-    if (w8 <= 128) ND_QR(8, 1, 128);
-    else if (w8 <= 256) ND_QR(8, 2, 128);
-    else if (w8 <= 512) ND_QR(8, 2, 256);
-    else if (w8 <= 1024) ND_QR(8, 2, 512);
-    else ND_QR(8, 3, 512);
-  } else {
-    if (cols <= 1024) ND_QR(1, 4, 256);
-    else if (cols <= 4096) ND_QR(1, 16, 256);
-    else ND_QR(1, 16, 512);
-  }
-#undef ND_QR
-  ND_CUDA(cudaGetLastError());
-  return ND_OK;
+  if (dtype == ND_F32) return launch<ND_F32>(x, rows, cols, ldx, q, ldq, scale, stream);
+  if (dtype == ND_F16) return launch<ND_F16>(x, rows, cols, ldx, q, ldq, scale, stream);
+  return launch<ND_BF16>(x, rows, cols, ldx, q, ldq, scale, stream);
 }
 
 }  // namespace nd

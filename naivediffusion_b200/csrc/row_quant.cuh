@@ -44,10 +44,4 @@ __device__ __forceinline__ uint32_t pack_low_bytes(uint32_t a, uint32_t b, uint3
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-// Four values, already scaled to [-127, 127].
-__device__ __forceinline__ uint32_t pack_rint(float a, float b, float c, float d) {
-  return pack_low_bytes(__float_as_uint(a + kRintMagic), __float_as_uint(b + kRintMagic), __float_as_uint(c + kRintMagic),
-                        __float_as_uint(d + kRintMagic));
-}
-
 }  // namespace nd

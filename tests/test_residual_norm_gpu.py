@@ -43,7 +43,8 @@ def _check_y(got, y, dy, out):
 
 
 @pytest.mark.parametrize("rows,width", [(1, 1), (1, 1024), (3, 4), (5, 130), (37, 512), (129, 1155), (64, 2048), (33, 3584),
-                                        (7, 4100), (4, 8192), (3, 12289), (2, 16384)])
+                                        (7, 4100), (4, 8192), (3, 12289), (2, 16384), (1300, 1032), (1501, 2048), (1250, 2064),
+                                        (1193, 4096), (1210, 8192), (1400, 1028), (1700, 900)])
 @pytest.mark.parametrize("btype,out,post,pre", [(BF16, BF16, RMS, RMS), (F16, I8, NONE, LAYER), (F32, F32, LAYER, LAYER),
                                                 (None, F16, NONE, RMS)])
 def test_against_64_bits(cuda, rows, width, btype, out, post, pre):
