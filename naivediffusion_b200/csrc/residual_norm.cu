@@ -44,88 +44,104 @@ struct ResidualNorm {
   float residual_scale, plus_one, eps, inv_width;
 };
 
-template <int VEC>
-struct Vals {
-  float f[VEC];
+// A thread's share of a row: V groups of VEC neighbouring columns, T * VEC
+// apart, as pairs for the paired fp32 instructions (VEC = 1: two groups make a
+// pair). Pointers are to the thread's first column, so every offset is a
+// constant; `rem` is the width less that column. Columns at and past the width
+// load as 0.
+template <int VEC, int V, int T>
+struct Share {
+  static constexpr int H = VEC * V / 2;
+  static constexpr int kStep = VEC * T;
+
+  template <bool ONCE>  // read once from global memory: past L1
+  static __device__ __forceinline__ void load(const float* p, int rem, float2 (&v)[H]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if constexpr (VEC == 4) {
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (kStep * i < rem) {
+          if constexpr (ONCE)
+            asm volatile("ld.global.L1::no_allocate.v4.f32 {%0,%1,%2,%3}, [%4];"
+                         : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+                         : "l"(p + kStep * i));
+          else
+            x = *reinterpret_cast<const float4*>(p + kStep * i);
+        }
+        v[2 * i] = make_float2(x.x, x.y);
+        v[2 * i + 1] = make_float2(x.z, x.w);
+      } else {
+        (i & 1 ? v[i / 2].y : v[i / 2].x) = kStep * i < rem ? p[kStep * i] : 0.f;
+      }
+    }
+  }
+  template <bool F16>
+  static __device__ __forceinline__ void load(const uint16_t* p, int rem, float2 (&v)[H]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if constexpr (VEC == 4) {
+        uint2 w = make_uint2(0u, 0u);
+        if (kStep * i < rem) w = *reinterpret_cast<const uint2*>(p + kStep * i);
+        v[2 * i] = halves<F16>(w.x);
+        v[2 * i + 1] = halves<F16>(w.y);
+      } else {
+        const uint32_t w = kStep * i < rem ? p[kStep * i] : 0u;
+        (i & 1 ? v[i / 2].y : v[i / 2].x) = halves<F16>(w).x;
+      }
+    }
+  }
+  template <bool F16>
+  static __device__ __forceinline__ float2 halves(uint32_t w) {
+    if constexpr (F16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+    else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  // From `p` + the thread's first column, element type `type`.
+  template <bool ONCE>
+  static __device__ __forceinline__ void load_typed(const void* p, int first, int type, int rem, float2 (&v)[H]) {
+    if (type == ND_F32) load<ONCE>(static_cast<const float*>(p) + first, rem, v);
+    else if (type == ND_F16) load<true>(static_cast<const uint16_t*>(p) + first, rem, v);
+    else load<false>(static_cast<const uint16_t*>(p) + first, rem, v);
+  }
+
+  static __device__ __forceinline__ void store(float* p, int rem, const float2 (&v)[H]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (kStep * i < rem) {
+        if constexpr (VEC == 4)
+          *reinterpret_cast<float4*>(p + kStep * i) = make_float4(v[2 * i].x, v[2 * i].y, v[2 * i + 1].x, v[2 * i + 1].y);
+        else p[kStep * i] = i & 1 ? v[i / 2].y : v[i / 2].x;
+      }
+  }
+  template <bool F16>
+  static __device__ __forceinline__ void store(uint16_t* p, int rem, const float2 (&v)[H]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (kStep * i < rem) {
+        if constexpr (VEC == 4) {
+          const float2 a = v[2 * i], b = v[2 * i + 1];
+          *reinterpret_cast<uint2*>(p + kStep * i) = F16 ? make_uint2(pack_f16(a.x, a.y), pack_f16(b.x, b.y))
+                                                         : make_uint2(pack_bf16(a.x, a.y), pack_bf16(b.x, b.y));
+        } else {
+          const float f = i & 1 ? v[i / 2].y : v[i / 2].x;
+          p[kStep * i] = static_cast<uint16_t>(F16 ? pack_f16(f, 0.f) : pack_bf16(f, 0.f));
+        }
+      }
+  }
+  // The low bytes of v's bit patterns.
+  static __device__ __forceinline__ void store(int8_t* p, int rem, const float2 (&v)[H]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (kStep * i < rem) {
+        if constexpr (VEC == 4)
+          *reinterpret_cast<uint32_t*>(p + kStep * i) =
+              pack_low_bytes(__float_as_uint(v[2 * i].x), __float_as_uint(v[2 * i].y), __float_as_uint(v[2 * i + 1].x),
+                             __float_as_uint(v[2 * i + 1].y));
+        else p[kStep * i] = static_cast<int8_t>(__float_as_uint(i & 1 ? v[i / 2].y : v[i / 2].x) & 0xffu);
+      }
+  }
 };
 
-// Element by element; four at a time as two paired operations.
-template <int VEC>
-__device__ __forceinline__ Vals<VEC> mul(const Vals<VEC>& a, const Vals<VEC>& b) {
-  Vals<VEC> r;
-  if constexpr (VEC == 4) {
-#pragma unroll
-    for (int j = 0; j < 4; j += 2) {
-      const float2 t = fmul2(make_float2(a.f[j], a.f[j + 1]), make_float2(b.f[j], b.f[j + 1]));
-      r.f[j] = t.x;
-      r.f[j + 1] = t.y;
-    }
-  } else {
-    r.f[0] = a.f[0] * b.f[0];
-  }
-  return r;
-}
-template <int VEC>
-__device__ __forceinline__ Vals<VEC> fma(const Vals<VEC>& a, const Vals<VEC>& b, const Vals<VEC>& c) {
-  Vals<VEC> r;
-  if constexpr (VEC == 4) {
-#pragma unroll
-    for (int j = 0; j < 4; j += 2) {
-      const float2 t = ffma2(make_float2(a.f[j], a.f[j + 1]), make_float2(b.f[j], b.f[j + 1]), make_float2(c.f[j], c.f[j + 1]));
-      r.f[j] = t.x;
-      r.f[j + 1] = t.y;
-    }
-  } else {
-    r.f[0] = fmaf(a.f[0], b.f[0], c.f[0]);
-  }
-  return r;
-}
-template <int VEC>
-__device__ __forceinline__ Vals<VEC> all(float f) {
-  Vals<VEC> r;
-#pragma unroll
-  for (int j = 0; j < VEC; ++j) r.f[j] = f;
-  return r;
-}
-
-// VEC consecutive fp32 values that are read once (they stay out of L1).
-template <int VEC>
-__device__ __forceinline__ Vals<VEC> load_once(const float* p) {
-  Vals<VEC> r;
-  if constexpr (VEC == 4) {
-    asm volatile("ld.global.L1::no_allocate.v4.f32 {%0,%1,%2,%3}, [%4];"
-                 : "=f"(r.f[0]), "=f"(r.f[1]), "=f"(r.f[2]), "=f"(r.f[3])
-                 : "l"(p));
-  } else {
-    r.f[0] = *p;
-  }
-  return r;
-}
-
-template <int VEC>
-__device__ __forceinline__ Vals<VEC> load_branch(const void* p, long long i, int type) {
-  if (type == ND_F32) return load_once<VEC>(static_cast<const float*>(p) + i);
-  Vals<VEC> r;
-  if constexpr (VEC == 4) {
-    uint32_t a, b;
-    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];"
-                 : "=r"(a), "=r"(b)
-                 : "l"(static_cast<const uint16_t*>(p) + i));
-    float2 lo, hi;
-    if (type == ND_F16) {
-      lo = __half22float2(*reinterpret_cast<const __half2*>(&a));
-      hi = __half22float2(*reinterpret_cast<const __half2*>(&b));
-    } else {
-      lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&a));
-      hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&b));
-    }
-    r.f[0] = lo.x; r.f[1] = lo.y; r.f[2] = hi.x; r.f[3] = hi.y;
-  } else {
-    r.f[0] = type == ND_F16 ? __half2float(static_cast<const __half*>(p)[i])
-                            : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-  }
-  return r;
-}
+__device__ __forceinline__ float2 splat(float f) { return make_float2(f, f); }
 
 constexpr int kMaxSlots = 8;
 
@@ -135,57 +151,6 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"(src), "r"(bytes), "r"(bar)
                : "memory");
-}
-
-// Four branch values from shared memory.
-__device__ __forceinline__ Vals<4> shared_branch(const uint8_t* p, int c, int type) {
-  Vals<4> r;
-  if (type == ND_F32) {
-    const float4 t = *reinterpret_cast<const float4*>(p + c * 4);
-    r.f[0] = t.x; r.f[1] = t.y; r.f[2] = t.z; r.f[3] = t.w;
-  } else {
-    const uint2 t = *reinterpret_cast<const uint2*>(p + c * 2);
-    float2 lo, hi;
-    if (type == ND_F16) {
-      lo = __half22float2(*reinterpret_cast<const __half2*>(&t.x));
-      hi = __half22float2(*reinterpret_cast<const __half2*>(&t.y));
-    } else {
-      lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&t.x));
-      hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&t.y));
-    }
-    r.f[0] = lo.x; r.f[1] = lo.y; r.f[2] = hi.x; r.f[3] = hi.y;
-  }
-  return r;
-}
-
-template <int VEC>
-__device__ __forceinline__ Vals<VEC> load_vec(const float* p) {
-  Vals<VEC> r;
-  if constexpr (VEC == 4) {
-    const float4 t = __ldg(reinterpret_cast<const float4*>(p));
-    r.f[0] = t.x; r.f[1] = t.y; r.f[2] = t.z; r.f[3] = t.w;
-  } else {
-    r.f[0] = __ldg(p);
-  }
-  return r;
-}
-
-// VEC values as out_type (ND_F32, ND_F16 or ND_BF16) at element i.
-template <int VEC>
-__device__ __forceinline__ void store_vals(void* p, long long i, const Vals<VEC>& v, int type) {
-  if constexpr (VEC == 4) {
-    if (type == ND_F32) {
-      *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(v.f[0], v.f[1], v.f[2], v.f[3]);
-    } else {
-      const uint2 w = type == ND_F16 ? make_uint2(pack_f16(v.f[0], v.f[1]), pack_f16(v.f[2], v.f[3]))
-                                     : make_uint2(pack_bf16(v.f[0], v.f[1]), pack_bf16(v.f[2], v.f[3]));
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = w;
-    }
-  } else {
-    if (type == ND_F32) static_cast<float*>(p)[i] = v.f[0];
-    else if (type == ND_F16) static_cast<__half*>(p)[i] = __float2half_rn(v.f[0]);
-    else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v.f[0]);
-  }
 }
 
 // Sum / maximum over the T threads of a row, in a fixed order. `slot`: this
@@ -216,65 +181,43 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* slot) {
   return v;
 }
 
-// The per-column factors of the VEC columns from c: the branch's post weight
-// times gate, y's pre weight times (1 + scale), and the shift.
-template <int VEC>
-__device__ __forceinline__ Vals<VEC> factor(const float* weight, float plus_one, const float* vec, float plus, int c) {
-  Vals<VEC> k;
-#pragma unroll
-  for (int j = 0; j < VEC; ++j) k.f[j] = 1.f;
-  if (weight) {
-    const Vals<VEC> w = load_vec<VEC>(weight + c);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) k.f[j] = w.f[j] + plus_one;
-  }
-  if (vec) {
-    const Vals<VEC> w = load_vec<VEC>(vec + c);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) k.f[j] *= w.f[j] + plus;
-  }
-  return k;
-}
-// Read where they are used, or held in registers from row to row.
+// A thread's per-column factors for vector set offset `vec`: the branch's post
+// weight times gate, y's pre weight times (1 + scale), and the shift. Held from
+// row to row, or (lazy) read where they are used.
 template <int VEC, int V, int T>
-struct LazyFactors {
-  const ResidualNorm& a;
-  long long vec;
-  int t;
-  __device__ __forceinline__ int col(int i) const { return (t + T * i) * VEC; }
-  __device__ __forceinline__ Vals<VEC> branch(int i) const {
-    return factor<VEC>(a.post_weight, a.plus_one, a.gate ? a.gate + vec : nullptr, 0.f, col(i));
-  }
-  __device__ __forceinline__ Vals<VEC> y(int i) const {
-    return factor<VEC>(a.pre_weight, a.plus_one, a.scale ? a.scale + vec : nullptr, 1.f, col(i));
-  }
-  __device__ __forceinline__ Vals<VEC> shift(int i) const {
-    Vals<VEC> k;
+struct Factors {
+  using S = Share<VEC, V, T>;
+  static __device__ __forceinline__ void product(const float* weight, float plus_one, const float* vec, float plus, int rem,
+                                                 float2 (&k)[S::H]) {
+    if (weight) {
+      S::template load<false>(weight, rem, k);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) k.f[j] = 0.f;
-    return a.shift ? load_vec<VEC>(a.shift + vec + col(i)) : k;
-  }
-};
-template <int VEC, int V, int T>
-struct HeldFactors {
-  Vals<VEC> b[V], s[V], h[V];
-  __device__ __forceinline__ void load(const ResidualNorm& a, long long vec, int t) {
-    const LazyFactors<VEC, V, T> lazy{a, vec, t};
+      for (int h = 0; h < S::H; ++h) k[h] = fadd2(k[h], splat(plus_one));
+    } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      if (lazy.col(i) < a.width) {
-        b[i] = lazy.branch(i);
-        s[i] = lazy.y(i);
-        h[i] = lazy.shift(i);
-      } else {
+      for (int h = 0; h < S::H; ++h) k[h] = splat(1.f);
+    }
+    if (vec) {
+      float2 g[S::H];
+      S::template load<false>(vec, rem, g);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) b[i].f[j] = s[i].f[j] = h[i].f[j] = 0.f;
-      }
+      for (int h = 0; h < S::H; ++h) k[h] = fmul2(k[h], fadd2(g[h], splat(plus)));
     }
   }
-  __device__ __forceinline__ Vals<VEC> branch(int i) const { return b[i]; }
-  __device__ __forceinline__ Vals<VEC> y(int i) const { return s[i]; }
-  __device__ __forceinline__ Vals<VEC> shift(int i) const { return h[i]; }
+  static __device__ __forceinline__ const float* at(const float* p, long long i) { return p ? p + i : nullptr; }
+  static __device__ __forceinline__ void branch(const ResidualNorm& a, long long vec, int first, float2 (&k)[S::H]) {
+    product(at(a.post_weight, first), a.plus_one, at(a.gate, vec + first), 0.f, a.width - first, k);
+  }
+  static __device__ __forceinline__ void y(const ResidualNorm& a, long long vec, int first, float2 (&k)[S::H],
+                                           float2 (&shift)[S::H]) {
+    product(at(a.pre_weight, first), a.plus_one, at(a.scale, vec + first), 1.f, a.width - first, k);
+    if (a.shift) {
+      S::template load<false>(a.shift + vec + first, a.width - first, shift);
+    } else {
+#pragma unroll
+      for (int h = 0; h < S::H; ++h) shift[h] = splat(0.f);
+    }
+  }
 };
 
 // The vector set of row r, as an offset, and the first row past its share.
@@ -284,100 +227,102 @@ __device__ __forceinline__ long long vec_of(const ResidualNorm& a, int r, int* e
   return i * a.vec_stride;
 }
 
-// sum over pairs of a thread's values: f32x2 where there are four at a time.
-template <int VEC, int V, bool SQUARE>
-__device__ __forceinline__ float thread_sum(const Vals<VEC> (&w)[V]) {
-  if constexpr (VEC == 4) {
-    float2 s = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; j += 2) {
-        const float2 p = make_float2(w[i].f[j], w[i].f[j + 1]);
-        s = SQUARE ? ffma2(p, p, s) : fadd2(s, p);
-      }
-    return s.x + s.y;
-  } else {
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) s = SQUARE ? fmaf(w[i].f[0], w[i].f[0], s) : s + w[i].f[0];
-    return s;
-  }
-}
-
-// One row, held by T threads as V x VEC values each (columns at and past the
-// width are 0 in v and b): x' and y. `red`: five reductions' words.
-template <int VEC, int V, int T, typename Factors>
-__device__ __forceinline__ void finish_row(const ResidualNorm& a, long long r, int t, Vals<VEC> (&v)[V],
-                                           Vals<VEC> (&b)[V], const Factors& k, float (*red)[T / 32]) {
-  auto col = [&](int i) { return (t + T * i) * VEC; };
+// One row in T threads' registers: x' and y. `red`: five reductions' words.
+// held: this row's factors, or null to read them here.
+template <int VEC, int V, int T>
+struct HeldFactors {
+  float2 branch[VEC * V / 2], y[VEC * V / 2], shift[VEC * V / 2];
+};
+template <int VEC, int V, int T>
+__device__ __forceinline__ void finish_row(const ResidualNorm& a, long long r, int t, float2 (&v)[VEC * V / 2],
+                                           float2 (&b)[VEC * V / 2], const HeldFactors<VEC, V, T>* held, long long vec,
+                                           float (*red)[T / 32]) {
+  using S = Share<VEC, V, T>;
+  const int first = t * VEC, rem = a.width - first;
   // Subtract the mean (LayerNorm), then return rsqrt(mean square + eps).
-  auto normalize = [&](Vals<VEC> (&w)[V], int kind, int slot) {
+  auto normalize = [&](float2 (&w)[S::H], int kind, int slot) {
     if (kind == ND_NORM_LAYER) {
-      const float mean = row_sum<T>(thread_sum<VEC, V, false>(w), red[slot]) * a.inv_width;
+      float2 s = splat(0.f);
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (col(i) < a.width) w[i] = fma(w[i], all<VEC>(1.f), all<VEC>(-mean));
+      for (int h = 0; h < S::H; ++h) s = fadd2(s, w[h]);
+      const float mean = row_sum<T>(s.x + s.y, red[slot]) * a.inv_width;
+#pragma unroll
+      for (int i = 0; i < V; ++i)  // columns past the width stay 0
+        if (S::kStep * i < rem) {
+          if constexpr (VEC == 4) {
+            w[2 * i] = fadd2(w[2 * i], splat(-mean));
+            w[2 * i + 1] = fadd2(w[2 * i + 1], splat(-mean));
+          } else {
+            (i & 1 ? w[i / 2].y : w[i / 2].x) -= mean;
+          }
+        }
     }
-    return rsqrtf(fmaf(row_sum<T>(thread_sum<VEC, V, true>(w), red[slot + 1]), a.inv_width, a.eps));
+    float2 q = splat(0.f);
+#pragma unroll
+    for (int h = 0; h < S::H; ++h) q = ffma2(w[h], w[h], q);
+    return rsqrtf(fmaf(row_sum<T>(q.x + q.y, red[slot + 1]), a.inv_width, a.eps));
   };
 
+  const float2 alpha = splat(a.residual_scale);
   if (a.branch) {
-    const float rstd = a.post != ND_NORM_NONE ? normalize(b, a.post, 0) : 1.f;
+    const float2 rstd = splat(a.post != ND_NORM_NONE ? normalize(b, a.post, 0) : 1.f);
+    float2 own[S::H];
+    if (!held) Factors<VEC, V, T>::branch(a, vec, first, own);
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (col(i) < a.width) v[i] = fma(mul(b[i], all<VEC>(rstd)), k.branch(i), mul(v[i], all<VEC>(a.residual_scale)));
+    for (int h = 0; h < S::H; ++h) v[h] = ffma2(fmul2(b[h], rstd), held ? held->branch[h] : own[h], fmul2(v[h], alpha));
   } else if (a.residual_scale != 1.f) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = mul(v[i], all<VEC>(a.residual_scale));
+    for (int h = 0; h < S::H; ++h) v[h] = fmul2(v[h], alpha);
   }
-  if (a.x_out) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = col(i);
-      if (c < a.width) store_vals<VEC>(a.x_out, r * a.ldxo + c, v[i], ND_F32);
-    }
-  }
+  if (a.x_out) S::store(a.x_out + r * a.ldxo + first, rem, v);
   if (!a.y) return;
 
-  const float rstd = a.pre != ND_NORM_NONE ? normalize(v, a.pre, 2) : 1.f;
+  const float2 rstd = splat(a.pre != ND_NORM_NONE ? normalize(v, a.pre, 2) : 1.f);
+  if (held) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int c = col(i);
-    if (c < a.width) {
-      v[i] = fma(mul(v[i], all<VEC>(rstd)), k.y(i), k.shift(i));
-      if (a.out_type != ND_I8) store_vals<VEC>(a.y, r * a.ldy + c, v[i], a.out_type);
-    }
+    for (int h = 0; h < S::H; ++h) v[h] = ffma2(fmul2(v[h], rstd), held->y[h], held->shift[h]);
+  } else {
+    float2 k[S::H], shift[S::H];
+    Factors<VEC, V, T>::y(a, vec, first, k, shift);
+#pragma unroll
+    for (int h = 0; h < S::H; ++h) v[h] = ffma2(fmul2(v[h], rstd), k[h], shift[h]);
   }
-  if (a.out_type != ND_I8) return;
+  if (a.out_type == ND_BF16) {
+    S::template store<false>(static_cast<uint16_t*>(a.y) + r * a.ldy + first, rem, v);
+    return;
+  }
+  if (a.out_type == ND_F16) {
+    S::template store<true>(static_cast<uint16_t*>(a.y) + r * a.ldy + first, rem, v);
+    return;
+  }
+  if (a.out_type == ND_F32) {
+    S::store(static_cast<float*>(a.y) + r * a.ldy + first, rem, v);
+    return;
+  }
+  // int8. Columns past the width: their factors are anything, their bits not counted.
   uint32_t peak = 0u;
 #pragma unroll
   for (int i = 0; i < V; ++i)
-    if (col(i) < a.width)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) peak = max(peak, abs_bits(v[i].f[j]));
+    if (S::kStep * i < rem) {
+      if constexpr (VEC == 4)
+        peak = max(max(peak, max(abs_bits(v[2 * i].x), abs_bits(v[2 * i].y))),
+                   max(abs_bits(v[2 * i + 1].x), abs_bits(v[2 * i + 1].y)));
+      else peak = max(peak, abs_bits(i & 1 ? v[i / 2].y : v[i / 2].x));
+    }
   // y is an fp32 result already, so the quotient's last bit decides nothing
   // that fp32 had not rounded before: multiply by 127 / peak.
   const RowScale s = row_scale(row_max<T>(peak, reinterpret_cast<uint32_t*>(red[4])));
   if (t == 0) a.y_scale[r] = s.scale;
-  int8_t* y = static_cast<int8_t*>(a.y) + r * a.ldy;
   // Where 127 / peak leaves fp32's range, both are first multiplied up.
-  const float shift = s.peak < 1e-30f ? 0x1p96f : 1.f;
-  const float inverse = s.inverse == 0.f || shift == 1.f ? s.inverse : __fdiv_rn(127.0f, s.peak * shift);
+  const bool tiny = s.inverse != 0.f && s.peak < 1e-30f;
+  const float inverse = tiny ? __fdiv_rn(127.0f, s.peak * 0x1p96f) : s.inverse;
+  if (tiny) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int c = col(i);
-    if (c < a.width) {
-      Vals<VEC> q = v[i];
-      if (shift != 1.f) q = mul(q, all<VEC>(shift));
-      q = fma(inverse != 0.f ? q : all<VEC>(0.f), all<VEC>(inverse), all<VEC>(kRintMagic));
-      if constexpr (VEC == 4)
-        *reinterpret_cast<uint32_t*>(y + c) = pack_low_bytes(__float_as_uint(q.f[0]), __float_as_uint(q.f[1]),
-                                                             __float_as_uint(q.f[2]), __float_as_uint(q.f[3]));
-      else
-        y[c] = static_cast<int8_t>(__float_as_uint(q.f[0]) & 0xffu);
-    }
+    for (int h = 0; h < S::H; ++h) v[h] = fmul2(v[h], splat(0x1p96f));
   }
+#pragma unroll
+  for (int h = 0; h < S::H; ++h) v[h] = s.inverse != 0.f ? ffma2(v[h], splat(inverse), splat(kRintMagic)) : splat(kRintMagic);
+  S::store(static_cast<int8_t*>(a.y) + r * a.ldy + first, rem, v);
 }
 
 // One row per T threads, loaded straight into registers: few rows, narrow
@@ -387,23 +332,46 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T) residual_norm_kernel(const 
   griddep_launch();
   griddep_wait();
   __shared__ float red[5][T / 32];
+  using S = Share<VEC, V, T>;
   constexpr int kRows = T < 128 ? 128 / T : 1;
   const int t = threadIdx.x % T;
   const int row = blockIdx.x * kRows + threadIdx.x / T;
   if (row >= a.rows) return;  // whole warps: only T = 32 has several rows per block
   const long long r = row;
-  Vals<VEC> v[V], b[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int c = (t + T * i) * VEC;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) v[i].f[j] = b[i].f[j] = 0.f;
-    if (c < a.width) {
-      v[i] = load_once<VEC>(a.x + r * a.ldx + c);
-      if (a.branch) b[i] = load_branch<VEC>(a.branch, r * a.ldb + c, a.branch_type);
-    }
+  float2 v[S::H], b[S::H];
+  S::template load<true>(a.x + r * a.ldx + t * VEC, a.width - t * VEC, v);
+  if (a.branch) {
+    const uint8_t* p = static_cast<const uint8_t*>(a.branch) + r * a.ldb * (a.branch_type == ND_F32 ? 4 : 2);
+    S::template load_typed<true>(p, t * VEC, a.branch_type, a.width - t * VEC, b);
   }
-  finish_row<VEC, V, T>(a, r, t, v, b, LazyFactors<VEC, V, T>{a, vec_of(a, row), t}, red);
+  finish_row<VEC, V, T>(a, r, t, v, b, nullptr, vec_of(a, row), red);
+}
+
+// The part of one row that a bulk copy takes: from the 16-byte boundary at or
+// before its first byte to the one at or after its last, except where that
+// would leave the matrix (rows at its ends that start or end off a boundary);
+// those few bytes are copied by hand.
+struct RowSpan {
+  const uint8_t* start;  // of the row
+  uint32_t skip;         // bytes between the 16-byte boundary before it and the row: its place in its buffer
+  uint32_t head, tail;   // bytes of the row to copy by hand at either end
+};
+__device__ __forceinline__ RowSpan row_span(const uint8_t* start, const uint8_t* first, const uint8_t* last, uint32_t bytes) {
+  RowSpan s;  // first, last: the matrix
+  s.start = start;
+  s.skip = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(start) & 15u);
+  const uint32_t end = (s.skip + bytes) & 15u;  // bytes past the last boundary inside the row's end
+  s.head = s.skip && start - s.skip < first ? min(16u - s.skip, bytes) : 0u;
+  s.tail = end && start + bytes + (16u - end) > last ? min(end, bytes - s.head) : 0u;
+  return s;
+}
+// Ask for the row into `dst` (16-byte aligned, bytes + 30 long); returns the
+// bytes that the bulk copy brings. Called by one thread, before it arrives.
+__device__ __forceinline__ uint32_t span_bulk(const RowSpan& s, uint32_t bytes, uint32_t& from) {
+  from = s.head ? 16u : 0u;  // the copy's first byte in the buffer
+  const uint32_t all = (s.skip + bytes + 15u) & ~15u;
+  const uint32_t to = s.tail ? (s.skip + bytes) & ~15u : all;
+  return to > from ? to - from : 0u;
 }
 
 // Many rows: persistent blocks of T threads, each working through rows
@@ -412,17 +380,21 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T) residual_norm_kernel(const 
 // row per block straight into registers ran at 55 % of the copy rate at
 // 4352 x 4096: the loads paused while the rows were reduced and written). The
 // thread's columns are the same in every row, so the per-column factors stay
-// in registers and are read again only where the vector set changes.
-template <int V, int T, int CTAS>
-__global__ void __launch_bounds__(T, CTAS) residual_norm_ring_kernel(const ResidualNorm a, int slots, unsigned* status) {
+// in registers and are read again only where the vector set changes. VEC = 1:
+// rows of any width and alignment, shared memory and stores one value at a
+// time.
+template <int VEC, int V, int T, int CTAS>
+__global__ void __launch_bounds__(T, CTAS) residual_norm_ring_kernel(const ResidualNorm a, int slots, uint32_t x_room,
+                                                                     uint32_t b_room, unsigned* status) {
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ float red[5][T / 32];
   __shared__ uint64_t full_bars[kMaxSlots];
   __shared__ volatile int abort_flag;
   const int t = threadIdx.x;
+  const int b_elem = a.branch_type == ND_F32 ? 4 : 2;
   const uint32_t x_bytes = a.width * 4u;
-  const uint32_t b_bytes = a.branch ? a.width * (a.branch_type == ND_F32 ? 4u : 2u) : 0u;
-  const uint32_t slot_bytes = x_bytes + b_bytes;
+  const uint32_t b_bytes = a.branch ? static_cast<uint32_t>(a.width * b_elem) : 0u;
+  const uint32_t slot_bytes = x_room + b_room;
   const uint32_t base = smem_u32(ring);
   if (t == 0) {
     for (int s = 0; s < slots; ++s) mbar_init(smem_u32(&full_bars[s]), 1);
@@ -432,20 +404,57 @@ __global__ void __launch_bounds__(T, CTAS) residual_norm_ring_kernel(const Resid
   __syncthreads();
   griddep_launch();
   griddep_wait();
-  auto fetch = [&](int row, int s) {
-    const long long r = row;  // one thread
-    const uint32_t bar = smem_u32(&full_bars[s]), dst = base + s * slot_bytes;
-    mbar_arrive_expect_tx(bar, slot_bytes);
-    bulk_load(dst, a.x + r * a.ldx, x_bytes, bar);
-    if (b_bytes)
-      bulk_load(dst + x_bytes, static_cast<const uint8_t*>(a.branch) + r * a.ldb * (a.branch_type == ND_F32 ? 4 : 2), b_bytes, bar);
-  };
+  // Thread 0 asks for rows: the next one, where it starts, and the slot it goes to.
   const int step = gridDim.x;
-  int next = blockIdx.x;  // thread 0: the next row to ask for
+  int next = blockIdx.x;
+  const uint8_t* next_x = reinterpret_cast<const uint8_t*>(a.x + next * a.ldx);
+  const uint8_t* next_b = static_cast<const uint8_t*>(a.branch) + (b_bytes ? next * a.ldb * b_elem : 0);
+  const long long x_step = step * a.ldx * 4, b_step = b_bytes ? step * a.ldb * b_elem : 0;
+  bool dirty = false;
+  auto fetch = [&](int s) {
+    const uint32_t bar = smem_u32(&full_bars[s]), dst = base + s * slot_bytes;
+    if constexpr (VEC == 4) {
+      mbar_arrive_expect_tx(bar, x_bytes + b_bytes);
+      bulk_load(dst, next_x, x_bytes, bar);
+      if (b_bytes) bulk_load(dst + x_room, next_b, b_bytes, bar);
+    } else {
+      uint32_t from_x, from_b = 0, n_b = 0;
+      const uint8_t* fx = reinterpret_cast<const uint8_t*>(a.x);
+      const RowSpan x = row_span(next_x, fx, fx + (a.rows - 1) * a.ldx * 4 + x_bytes, x_bytes);
+      const uint32_t n_x = span_bulk(x, x_bytes, from_x);
+      RowSpan b{};
+      if (b_bytes) {
+        const uint8_t* fb = static_cast<const uint8_t*>(a.branch);
+        b = row_span(next_b, fb, fb + (a.rows - 1) * a.ldb * b_elem + b_bytes, b_bytes);
+        n_b = span_bulk(b, b_bytes, from_b);
+      }
+      auto by_hand = [&](const RowSpan& w, uint32_t at, uint32_t bytes) {
+        uint8_t* to = ring + at + w.skip;
+        for (uint32_t i = 0; i < w.head; i += 2)
+          *reinterpret_cast<uint16_t*>(to + i) = *reinterpret_cast<const uint16_t*>(w.start + i);
+        for (uint32_t i = bytes - w.tail; i < bytes; i += 2)
+          *reinterpret_cast<uint16_t*>(to + i) = *reinterpret_cast<const uint16_t*>(w.start + i);
+      };
+      // Bytes once copied by hand may lie where a later bulk copy goes.
+      if (dirty) fence_proxy_async_smem();
+      if (x.head | x.tail | b.head | b.tail) {
+        by_hand(x, s * slot_bytes, x_bytes);
+        by_hand(b, s * slot_bytes + x_room, b_bytes);
+        dirty = true;
+      }
+      mbar_arrive_expect_tx(bar, n_x + n_b);
+      if (n_x) bulk_load(dst + from_x, x.start - x.skip + from_x, n_x, bar);
+      if (n_b) bulk_load(dst + x_room + from_b, b.start - b.skip + from_b, n_b, bar);
+    }
+    next += step;
+    next_x += x_step;
+    next_b += b_step;
+  };
   if (t == 0)
-    for (int i = 0; i < slots && next < a.rows; ++i, next += step) fetch(next, i);
+    for (int i = 0; i < slots && next < a.rows; ++i) fetch(i);
 
-  HeldFactors<4, V, T> k;
+  using S = Share<VEC, V, T>;
+  HeldFactors<VEC, V, T> k;
   int vec_end = 0;  // first row past the held set's share
   int it = 0, s = 0;
   uint32_t parity = 0;
@@ -454,25 +463,22 @@ __global__ void __launch_bounds__(T, CTAS) residual_norm_ring_kernel(const Resid
     if (t < 32) ok = mbar_wait(smem_u32(&full_bars[s]), parity, &abort_flag, status, kStatusTimeoutProducer);
     if (!__syncthreads_and(ok)) break;
     // Everyone is done with the row before this one: its slot is filled again.
-    if (t == 0 && it > 0 && next < a.rows) {
-      fetch(next, s > 0 ? s - 1 : slots - 1);
-      next += step;
+    if (t == 0 && it > 0 && next < a.rows) fetch(s > 0 ? s - 1 : slots - 1);
+    if (r >= vec_end) {
+      const long long vec = vec_of(a, r, &vec_end);
+      Factors<VEC, V, T>::branch(a, vec, t * VEC, k.branch);
+      Factors<VEC, V, T>::y(a, vec, t * VEC, k.y, k.shift);
     }
-    if (r >= vec_end) k.load(a, vec_of(a, r, &vec_end), t);
-    Vals<4> v[V], b[V];
-    const uint8_t* slot = ring + s * slot_bytes;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = (t + T * i) * 4;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[i].f[j] = b[i].f[j] = 0.f;
-      if (c < a.width) {
-        const float4 x = *reinterpret_cast<const float4*>(slot + c * 4);
-        v[i].f[0] = x.x; v[i].f[1] = x.y; v[i].f[2] = x.z; v[i].f[3] = x.w;
-        if (b_bytes) b[i] = shared_branch(slot + x_bytes, c, a.branch_type);
-      }
+    const uint8_t* x_row = ring + s * slot_bytes;
+    const uint8_t* b_row = x_row + x_room;
+    if constexpr (VEC == 1) {
+      x_row += reinterpret_cast<uintptr_t>(a.x + r * a.ldx) & 15u;
+      if (b_bytes) b_row += reinterpret_cast<uintptr_t>(static_cast<const uint8_t*>(a.branch) + r * a.ldb * b_elem) & 15u;
     }
-    finish_row<4, V, T>(a, r, t, v, b, k, red);
+    float2 v[S::H], b[S::H];
+    S::template load<false>(reinterpret_cast<const float*>(x_row) + t * VEC, a.width - t * VEC, v);
+    if (b_bytes) S::template load_typed<false>(b_row, t * VEC, a.branch_type, a.width - t * VEC, b);
+    finish_row<VEC, V, T>(a, r, t, v, b, &k, 0, red);
     if (++s == slots) {
       s = 0;
       parity ^= 1u;
@@ -502,10 +508,12 @@ int launch(const ResidualNorm& a, cudaStream_t stream) {
 
 // The ring kernel: CTAS blocks of T threads per SM, their rings sharing its
 // shared memory.
-template <int V, int T, int CTAS>
+template <int VEC, int V, int T, int CTAS>
 int launch_ring(const ResidualNorm& a, cudaStream_t stream) {
-  auto kernel = residual_norm_ring_kernel<V, T, CTAS>;
-  constexpr int kRing = 220 * 1024 / CTAS - 1024;  // the SM's 227 KB, less the blocks' static share and reserve
+  auto kernel = residual_norm_ring_kernel<VEC, V, T, CTAS>;
+  // The SM's 228 KB, less a block's reserve of 1 KB and its static share.
+  constexpr int kRing = (228 * 1024 / CTAS - 1024 - 512) & ~15;
+  static_assert(kRing + 512 <= 227 * 1024, "a block's most");
   static bool configured[64] = {};
   int dev = 0;
   ND_CUDA(cudaGetDevice(&dev));
@@ -513,14 +521,28 @@ int launch_ring(const ResidualNorm& a, cudaStream_t stream) {
     ND_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing));
     configured[dev & 63] = true;
   }
-  const int row_bytes = a.width * (4 + (a.branch ? (a.branch_type == ND_F32 ? 4 : 2) : 0));
-  const int slots = std::min(kMaxSlots, kRing / row_bytes);
+  // A row of any alignment lies up to 15 bytes past its buffer's start.
+  auto room = [](int bytes) { return VEC == 4 ? bytes : (bytes + 15 + 15) & ~15; };
+  const int x_room = room(a.width * 4);
+  const int b_room = a.branch ? room(a.width * (a.branch_type == ND_F32 ? 4 : 2)) : 0;
+  const int slots = std::min(kMaxSlots, kRing / (x_room + b_room));
   unsigned* status = device_status();
   if (!status) return fail(ND_ERR_CUDA, "residual_norm: no device status word");
   const unsigned grid = static_cast<unsigned>(std::min(a.rows, CTAS * sm_count()));
-  ND_CUDA(launch_pdl(kernel, dim3(grid), dim3(T), slots * row_bytes, stream, a, slots, status));
+  ND_CUDA(launch_pdl(kernel, dim3(grid), dim3(T), slots * (x_room + b_room), stream, a, slots,
+                     static_cast<uint32_t>(x_room), static_cast<uint32_t>(b_room), status));
   ND_CUDA(cudaGetLastError());
   return ND_OK;
+}
+
+template <int VEC>
+int launch_ring_for(const ResidualNorm& a, cudaStream_t stream) {  // width <= 8192
+  constexpr int V = 16 / VEC;
+  if (a.width <= 512) return launch_ring<VEC, V, 32, 14>(a, stream);
+  if (a.width <= 1024) return launch_ring<VEC, V, 64, 8>(a, stream);
+  if (a.width <= 2048) return launch_ring<VEC, V, 128, 4>(a, stream);
+  if (a.width <= 4096) return launch_ring<VEC, V, 256, 2>(a, stream);
+  return launch_ring<VEC, V, 512, 1>(a, stream);
 }
 
 bool aligned(const void* p, int64_t ld, int elem) {  // rows of 4 elements at once
@@ -585,21 +607,25 @@ int residual_norm(const nd_residual_norm_args& a, cudaStream_t stream) {
                    aligned(a.branch, a.ldb, elem_bytes(a.branch_dtype)) && aligned(a.y, a.ldy, elem_bytes(a.out_dtype)) &&
                    aligned(a.gate, vs, 4) && aligned(a.scale, vs, 4) && aligned(a.shift, vs, 4) &&
                    aligned(a.post_weight, 0, 4) && aligned(a.pre_weight, 0, 4);
+  // Bulk copies of whole rows take starts and lengths that are multiples of 16 bytes.
+  const bool bulk = by4 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 &&
+                    (!a.branch || (reinterpret_cast<uintptr_t>(a.branch) % 16 == 0 &&
+                                   (a.branch_dtype == ND_F32 || (a.width % 8 == 0 && a.ldb % 8 == 0))));
+  // Ring or straight into registers, us (both measured): 1500 x 4096 17.9 / 17.3, 4352 x 4096 39 / 46, 2048 x 1280
+  // 9.5 / 8.3, 16384 x 1024 37 / 38, 300 x 8192 10.7 / 12.2; unaligned 333 x 1155 5.7 / 4.7, 300 x 3001 8.5 / 12.3,
+  // 4000 x 3001 41 / 115.
+  const int64_t values = a.rows * a.width;
+  if (a.width <= 8192) {
+    if (bulk && (a.width > 4096 ? a.rows >= 2 * sm_count() : values >= (8 << 20))) return launch_ring_for<4>(k, stream);
+    if (!by4 && values >= 600000) return launch_ring_for<1>(k, stream);
+  }
   if (!by4) {
     if (a.width <= 1024) return launch<1, 4, 256>(k, stream);
-    if (a.width <= 4096) return launch<1, 16, 256>(k, stream);
+    if (a.width <= 2048) return launch<1, 8, 256>(k, stream);
+    if (a.width <= 8192) return launch<1, 8, 1024>(k, stream);
     return launch<1, 16, 1024>(k, stream);
   }
   const int64_t w4 = a.width / 4;
-  // Bulk copies take rows whose starts and lengths are multiples of 16 bytes.
-  const bool bulk = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 &&
-                    (!a.branch || (reinterpret_cast<uintptr_t>(a.branch) % 16 == 0 &&
-                                   (a.branch_dtype == ND_F32 || (a.width % 8 == 0 && a.ldb % 8 == 0))));
-  if (bulk && w4 > 256 && a.rows >= 8 * sm_count()) {
-    if (w4 <= 512) return launch_ring<4, 128, 4>(k, stream);
-    if (w4 <= 1024) return launch_ring<4, 256, 2>(k, stream);
-    if (w4 <= 2048) return launch_ring<4, 512, 1>(k, stream);
-  }
   if (w4 <= 128) return launch<4, 4, 32>(k, stream);
   if (w4 <= 256) return launch<4, 2, 128>(k, stream);
   if (w4 <= 512) return launch<4, 4, 128>(k, stream);

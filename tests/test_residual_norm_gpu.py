@@ -43,8 +43,8 @@ def _check_y(got, y, dy, out):
 
 
 @pytest.mark.parametrize("rows,width", [(1, 1), (1, 1024), (3, 4), (5, 130), (37, 512), (129, 1155), (64, 2048), (33, 3584),
-                                        (7, 4100), (4, 8192), (3, 12289), (2, 16384), (1300, 1032), (1501, 2048), (1250, 2064),
-                                        (1193, 4096), (1210, 8192), (1400, 1028), (1700, 900)])
+                                        (7, 4100), (4, 8192), (3, 12289), (2, 16384), (1400, 1028), (2500, 333), (1501, 1),
+                                        (1187, 2047), (305, 3001), (301, 8191), (310, 4104)])
 @pytest.mark.parametrize("btype,out,post,pre", [(BF16, BF16, RMS, RMS), (F16, I8, NONE, LAYER), (F32, F32, LAYER, LAYER),
                                                 (None, F16, NONE, RMS)])
 def test_against_64_bits(cuda, rows, width, btype, out, post, pre):
@@ -60,6 +60,24 @@ def test_against_64_bits(cuda, rows, width, btype, out, post, pre):
     kw["post"], kw["pre"] = kw.pop("post_norm"), kw.pop("pre_norm")
     xn, dx, y, dy = residual_norm64(x, b, **kw)
     check(new, xn, dx, "x'")
+    _check_y(got, y, dy, out)
+
+
+@pytest.mark.parametrize("rows,width,btype,out,post,pre,vecs", [
+    (8200, 1024, BF16, BF16, RMS, RMS, 3), (16500, 512, F16, F16, NONE, LAYER, 1), (4100, 2048, F32, I8, LAYER, RMS, 2),
+    (2100, 4096, BF16, I8, RMS, LAYER, 2), (1100, 8192, F32, F32, LAYER, LAYER, 2), (8200, 1032, None, BF16, NONE, LAYER, 4),
+    (30000, 296, BF16, F32, RMS, LAYER, 3000), (4300, 2047, BF16, F16, LAYER, LAYER, 5), (2300, 4095, F32, I8, NONE, RMS, 1)])
+def test_many_rows(cuda, rows, width, btype, out, post, pre, vecs):
+    """The rows that persistent blocks work through, in place, with many vector sets too."""
+    from naivediffusion_b200 import ops
+    x, b, v, w1, w2 = _inputs(rows, width, btype, vecs, rows + width)
+    per = -(-rows // vecs)
+    kw = dict(post_weight=w1 if post else None, gate=None if b is None else v[:, 0], residual_scale=1.0 if b is None else 0.5,
+              pre_weight=w2 if pre == RMS else None, scale=v[:, 1], shift=v[:, 2], rows_per_vec=per)
+    xn, dx, y, dy = residual_norm64(x, b, post=post, pre=pre, **kw)
+    got = ops.residual_norm(x, b, post_norm=post, pre_norm=pre, out_dtype=out, **kw)
+    ops.sync()
+    check(x, xn, dx, "x'")
     _check_y(got, y, dy, out)
 
 
@@ -100,27 +118,29 @@ def test_parts_alone(cuda):
     assert half is x and torch.equal(x, keep * 0.5)
 
 
-@pytest.mark.parametrize("offset,stride", [(0, 1284), (1, 1283), (4, 1300), (3, 1290)])
-def test_strides_and_alignment(cuda, offset, stride):
+@pytest.mark.parametrize("rows,width,offset,stride", [(21, 1280, 0, 1284), (21, 1280, 1, 1283), (21, 1280, 4, 1300),
+                                                      (21, 1280, 3, 1290), (6600, 1280, 8, 1296), (1300, 1280, 3, 1281),
+                                                      (1201, 517, 5, 517), (250001, 3, 1, 3), (90001, 7, 7, 9),
+                                                      (1250, 1030, 2, 1037), (600003, 1, 1, 1)])
+def test_strides_and_alignment(cuda, rows, width, offset, stride):
     """Rows of wider matrices, starting anywhere; what lies beside them stays."""
     from naivediffusion_b200 import ops
-    rows, width = 21, 1280
     g = _gen(offset + stride)
 
     def view(t):
         return t.as_strided((rows, width), (stride, 1), offset)
 
-    size = rows * stride + 8
+    size = rows * stride + 16
     xs, bs = _randn(g, size), _randn(g, size).to(BF16)
     v = 0.3 * _randn(g, 3, 4, width + 1)
     gate, scale, shift = (v[:, i, :width] for i in range(3))
     outs = {t: torch.full((size,), 7, device="cuda", dtype=t) for t in (F32, BF16, I8)}
     x2 = torch.full((size,), 7.0, device="cuda")
     xn, dx, y, dy = residual_norm64(view(xs), view(bs), post=RMS, gate=gate, pre=LAYER, scale=scale, shift=shift,
-                                    rows_per_vec=8)
+                                    rows_per_vec=(rows + 2) // 3)
     for dtype, store in outs.items():
         got = ops.residual_norm(view(xs), view(bs), x_out=view(x2), post_norm=RMS, gate=gate, scale=scale, shift=shift,
-                                rows_per_vec=8, out=view(store))
+                                rows_per_vec=(rows + 2) // 3, out=view(store))
         ops.sync()
         check(view(x2), xn, dx)
         _check_y(got, y, dy, dtype)
