@@ -179,7 +179,7 @@ def _norm(s):
                                 pre_weight=s["pre_weight"], scale=s["scale_vec"], shift=s["shift_vec"], rows_per_vec=per, eps=EPS,
                                 out_dtype=DTYPES[s["out"]])
         if s["out"] == "i8":
-            return {"x": got[0], "y": _values(got[1], got[2], torch.bfloat16), "scale": got[2]}
+            return {"x": got[0], "y": ops.dequantize(got[1].contiguous(), got[2], 0, torch.bfloat16), "scale": got[2]}
         return {"x": got[0], "y": got[1]}
     b = _plain_norm(s["branch_rows"].float(), s["post"])
     if s["post_weight"] is not None:
@@ -204,6 +204,7 @@ def _quantize(s):
     if own:
         from naivediffusion_b200 import ops
         q, scale = ops.quantize_rows(s["x"])
+        return {"values": ops.dequantize(q.contiguous(), scale, 0, to), "scale": scale}
     else:
         x = s["x"].double()  # values next to a half are rounded by their exact quotient
         peak = x.abs().amax(1, keepdim=True)
