@@ -549,11 +549,15 @@ int dequantize(const int8_t* q, const void* scales, int scale_dtype, int64_t qua
   if (out_dtype != ND_BF16 && out_dtype != ND_F16) return fail(ND_ERR_INVALID, "dequantize: out_dtype");
   const int64_t group = quant_group > 0 ? quant_group : cols;
   if (cols % group) return fail(ND_ERR_INVALID, "dequantize: quant_group must divide cols");
-  const long long total = rows * cols;
-  const unsigned grid = static_cast<unsigned>(std::min<long long>((total + 255) / 256, sm_count() * 16LL));
-  dequant_w8_kernel<<<grid, 256, 0, stream>>>(q, scales, scale_dtype == ND_F16, static_cast<int>(group),
-                                              static_cast<int>(cols / group), rows, static_cast<int>(cols),
-                                              out, out_dtype == ND_F16);
+  const bool by16 = cols % 16 == 0 && group % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 &&
+                    reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  const int64_t per_row = (cols + (by16 ? 16 * 128 : 128) - 1) / (by16 ? 16 * 128 : 128);  // blocks to cover a row at once
+  const int64_t most = sm_count() * 16LL;
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(rows, most)),
+                  static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(per_row, most / std::min<int64_t>(rows, most)))));
+  const int f16 = scale_dtype == ND_F16, g = static_cast<int>(group), sc = static_cast<int>(cols / group), w = static_cast<int>(cols);
+  if (by16) dequant_w8_kernel<16><<<grid, 128, 0, stream>>>(q, scales, f16, g, sc, rows, w, out, out_dtype == ND_F16);
+  else dequant_w8_kernel<1><<<grid, 128, 0, stream>>>(q, scales, f16, g, sc, rows, w, out, out_dtype == ND_F16);
   ND_CUDA(cudaGetLastError());
   return ND_OK;
 }

@@ -562,9 +562,12 @@ def dequantize(q: torch.Tensor, scales: torch.Tensor, quant_group: int = 32,
                out_dtype=torch.bfloat16) -> torch.Tensor:
     """w = round(q * scale) in out_dtype (DmlOps.Dequantize, Dml/DmlOps.cs:208-228)."""
     rows, cols = q.shape
-    out = torch.empty(rows, cols, device=q.device, dtype=out_dtype)
-    check(lib().nd_op_dequantize(q.data_ptr(), scales.data_ptr(), _DT[scales.dtype], quant_group, rows,
-                                 cols, out.data_ptr(), _DT[out_dtype], C.c_void_p(_stream())))
+    if not q.is_contiguous():
+        raise ValueError("dequantize: q must be contiguous")
+    device = q.device
+    out = torch.empty(rows, cols, device=device, dtype=out_dtype)
+    _launch("dequantize", device, lib().nd_op_dequantize, q.data_ptr(), scales.data_ptr(), _DT[scales.dtype], quant_group,
+            rows, cols, out.data_ptr(), _DT[out_dtype])
     return out
 
 

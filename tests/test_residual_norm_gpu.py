@@ -246,6 +246,20 @@ def test_quantize_rows_special_rows_and_strides(cuda):
         assert torch.equal(torch.isnan(scale), torch.isnan(ws)) and torch.equal(scale.nan_to_num(9), ws.nan_to_num(9))
 
 
+@pytest.mark.parametrize("rows,cols", [(1, 1), (77, 2048), (3000, 640), (1001, 5121), (9, 40000), (5000, 48)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_values_of_int8_rows(cuda, rows, cols, dtype):
+    """dequantize gives back what a quantized row stands for, rounded once: within half a step of x and of dtype."""
+    from naivediffusion_b200 import ops
+    x = _randn(_gen(rows + cols), rows, cols)
+    q, scale = ops.quantize_rows(x)
+    got = ops.dequantize(q.contiguous(), scale, 0, dtype)
+    ops.sync()
+    assert torch.equal(got, (q.float() * scale[:, None]).to(dtype))
+    v, s = x.double(), scale.double()[:, None]
+    check(got, v, s * 0.5 + 2 * U * v.abs() + half_step(v.abs() + s, dtype))
+
+
 def test_streams_and_graphs(cuda):
     """On a side stream, and captured: a replay reads the inputs' values of that moment."""
     from naivediffusion_b200 import ops

@@ -70,6 +70,11 @@ def test_linear_w8a8_refuses_wrong_operands():
             ops.linear_w8a8(*args, **kw)
 
 
+def test_dequantize_refuses_strided_rows():
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.dequantize(torch.zeros(8, 80, dtype=I8)[:, :72], torch.zeros(8), 0)
+
+
 def _refused(rc, text):
     assert rc in (_lib.ND_ERR_INVALID, _lib.ND_ERR_UNSUPPORTED), rc
     assert text in _lib.lib().nd_last_error().decode(), _lib.lib().nd_last_error()
