@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kI8PairThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(acc ? acce_leader1 : acce_leader0);
     }
-    if (lane == 0) bulk_wait<0>();
+    if (lane == 0) bulk_wait_read<0>();
     __syncwarp();
   }
 

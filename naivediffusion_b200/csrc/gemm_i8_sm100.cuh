@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(192, 1)
       }
       tc_fence_before();
     }
-    if (splits == 1 && lane == 0) bulk_wait<0>();
+    if (splits == 1 && lane == 0) bulk_wait_read<0>();
   }
   __syncwarp();
   tc_fence_before();
@@ -545,7 +545,7 @@ __global__ void __launch_bounds__(192, 1)
         }
         i8_chunk(args, &tmC, rows, row0, col0 + c * 32, c * 32, sx, r, r2, vecs, buf, sb, lane);
       }
-      if (lane == 0) bulk_wait<0>();
+      if (lane == 0) bulk_wait_read<0>();
       __syncwarp();
     }
     cluster_sync_all();  // no shared memory goes away while a peer reads it
