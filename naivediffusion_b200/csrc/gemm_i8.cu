@@ -237,8 +237,13 @@ int linear_w8a8(const nd_linear_w8a8_args& a, cudaStream_t stream) {
   if (a.rows <= kGemvI8Rows) return launch_i8_gemv(a, g, ldw, resid, stream);
 
   CUtensorMap ta, tb, tc;
-  if (a.rows <= kFewRows) {
-    const int nt = a.rows <= 16 ? 16 : 32;
+  // More tiles of 128 weight rows than SMs: half the stages, so that two CTAs
+  // share an SM and one's loads run under the other's start and end. That also
+  // takes 33 to 64 rows (otherwise the 128 x 128 tiles' vector epilogue is the
+  // faster one).
+  const bool two = (gated ? a.out_features / 64 : (n_all + 127) / 128) > sm_count();
+  if (a.rows <= kFewRows || (two && a.rows <= 2 * kFewRows)) {
+    const int nt = a.rows <= 16 ? 16 : a.rows <= 32 ? 32 : 64;
     int rc = make_tmap_2d(&ta, a.weight, 1, n_all, a.in_features, ldw, gated ? 16 : 128, 128, true);
     if (rc) return rc;
     rc = make_tmap_2d(&tb, a.x, 1, a.rows, a.in_features, a.ldx, nt, 128, true);
@@ -249,11 +254,9 @@ int linear_w8a8(const nd_linear_w8a8_args& a, cudaStream_t stream) {
     f.y = a.y;
     f.residual = a.residual;
     f.ld = resid ? a.ldr : a.ldy;
-    // More tiles than SMs: half the stages, so that two CTAs share an SM and
-    // one's loads run under the other's start and end.
-    const bool two = (gated ? a.out_features / 64 : (n_all + 127) / 128) > sm_count();
     if (nt == 16) return two ? launch_i8_few<16, 6>(ta, tb, f, stream) : launch_i8_few<16, 12>(ta, tb, f, stream);
-    return two ? launch_i8_few<32, 5>(ta, tb, f, stream) : launch_i8_few<32, 11>(ta, tb, f, stream);
+    if (nt == 32) return two ? launch_i8_few<32, 5>(ta, tb, f, stream) : launch_i8_few<32, 11>(ta, tb, f, stream);
+    return launch_i8_few<64, 4>(ta, tb, f, stream);
   }
   int rc = make_tmap_2d(&ta, a.x, 1, a.rows, a.in_features, a.ldx, 128, 128, true);
   if (rc) return rc;

@@ -33,7 +33,8 @@ def _case(m, n, k, seed, gated=False):
 
 SHAPES = [(1, 1, 1), (1, 8, 16), (1, 4096, 1024), (2, 1000, 4096), (3, 100, 130), (4, 640, 2048), (5, 256, 64), (8, 999, 1155),
           (16, 2560, 2048), (33, 72, 5000), (77, 1280, 2048), (128, 128, 128), (129, 257, 129), (154, 2560, 2048),
-          (300, 512, 96), (512, 4096, 1024), (1003, 999, 1155), (1024, 1024, 640), (1300, 2050, 320), (2049, 640, 2048)]
+          (300, 512, 96), (512, 4096, 1024), (9, 19001, 200), (27, 19500, 300), (40, 19003, 256), (64, 20000, 130),
+          (20, 256, 6000), (50, 640, 9000), (90, 1000, 7000), (200, 384, 12000), (1003, 999, 1155), (1024, 1024, 640), (1300, 2050, 320), (2049, 640, 2048)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -62,7 +63,49 @@ def test_activations(cuda, m, act, out):
     check(y, v, dv + half_step(v.abs() + dv, out), act)
 
 
-@pytest.mark.parametrize("m", [1, 4, 60, 400, 1500])
+@pytest.mark.parametrize("m", [3, 12, 32, 41, 64, 100])
+@pytest.mark.parametrize("act", ["swiglu", "geglu"])
+@pytest.mark.parametrize("n,k", [(9600, 190), (256, 5000)])
+def test_gated_wide_and_deep(cuda, m, act, n, k):
+    """Few rows of many outputs, and of few outputs with the k blocks split."""
+    from naivediffusion_b200 import ops
+    _, x, sx, w, sw, b = _case(m, n, k, m + n, gated=True)
+    y = ops.linear_w8a8(x, sx, w, sw, b, epilogue=EPI[act])
+    ops.sync()
+    v, dv = linear64(x, sx, w, sw, b, act)
+    check(y, v, dv + half_step(v.abs() + dv, BF16), act)
+
+
+@pytest.mark.parametrize("m,n,k", [(2, 64, 256), (9, 200, 300), (30, 128, 6000), (45, 256, 9000), (64, 19200, 128), (90, 256, 256)])
+@pytest.mark.parametrize("act", ["silu", "gelu_erf", "gate", "add_store"])
+def test_shared_weights_at_few_rows(cuda, m, n, k, act):
+    """Every kernel for few rows with a split between two biases and gates."""
+    from naivediffusion_b200 import ops
+    g, x, sx, w, sw, _ = _case(m, n, k, m + k)
+    split = m // 2
+    b, gate = torch.randn(2 * n, generator=g, device="cuda"), torch.randn(2 * n, generator=g, device="cuda")
+    r0 = torch.randn(m, n, generator=g, device="cuda")
+    addend = torch.randn(m, n, generator=g, device="cuda").to(BF16)
+    kw = dict(group_split=split, shared_weights=True, epilogue=EPI[act])
+    if act == "gate":
+        got = ops.linear_w8a8(x, sx, w, sw, b, residual=r0.clone(), gate=gate, **kw)
+    else:
+        got = ops.linear_w8a8(x, sx, w, sw, b, addend=addend if act == "add_store" else None, **kw)
+    ops.sync()
+    for rows, cols in ((slice(0, split), slice(0, n)), (slice(split, m), slice(n, 2 * n))):
+        v, dv = linear64(x[rows], sx[rows], w, sw, b[cols], act if act in ("silu", "gelu_erf") else "store")
+        if act == "gate":
+            f = gate[cols].double()
+            want = r0[rows].double() + v * f
+            check(got[rows], want, dv * f.abs() + U * (v * f).abs() * 1.01 + U * want.abs() + 1e-30, act)
+            continue
+        if act == "add_store":
+            v = v + addend[rows].double()
+            dv = dv + U * v.abs()
+        check(got[rows], v, dv + half_step(v.abs() + dv, BF16), act)
+
+
+@pytest.mark.parametrize("m", [1, 4, 20, 60, 400, 1500])
 def test_residual_epilogues_and_addend(cuda, m):
     from naivediffusion_b200 import ops
     n, k = 333, 770
@@ -139,7 +182,7 @@ def test_largest_sums_are_exact(cuda, m, n, k):
     assert torch.equal(y, want.expand(m, n))
 
 
-@pytest.mark.parametrize("m", [1, 50, 1200])
+@pytest.mark.parametrize("m", [1, 20, 50, 1200])
 def test_what_lies_beside_stays(cuda, m):
     """Rows and columns past the output, and int8 columns past in_features, are neither written nor read."""
     from naivediffusion_b200 import ops
@@ -157,7 +200,7 @@ def test_what_lies_beside_stays(cuda, m):
         assert store[m:].eq(7).all() and store[:, n:].eq(7).all()
 
 
-@pytest.mark.parametrize("m", [2, 90, 1100])
+@pytest.mark.parametrize("m", [2, 17, 90, 1100])
 def test_special_scales(cuda, m):
     """A row quantized from NaN or infinity has scale NaN and its outputs are NaN; a row of zeros gives the bias."""
     from naivediffusion_b200 import ops
@@ -174,7 +217,7 @@ def test_special_scales(cuda, m):
     assert torch.equal(y[0], b) and torch.isnan(y[1]).all() and torch.isfinite(y[2:]).all()
 
 
-@pytest.mark.parametrize("m", [1, 150, 1400])
+@pytest.mark.parametrize("m", [1, 24, 150, 1400])
 def test_streams_and_graphs(cuda, m):
     """Two products at once on two streams, and a captured one replayed on other values."""
     from naivediffusion_b200 import ops
