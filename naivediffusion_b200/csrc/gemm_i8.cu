@@ -15,7 +15,10 @@ namespace nd {
 namespace {
 
 constexpr int kMaxSplits = 8;  // the portable cluster size
-constexpr int kFewRows = 32;   // of gemm_i8_few_kernel
+// Rows of gemm_i8_few_kernel. Against the 128 x 128 tiles, us: 16 x 4096 x 12288
+// 12.4 / 19.8, 32 x 4096 x 4096 7.4 / 8.4, 48 x 4096 x 12288 14.5 / 14.5,
+// 64 x 4096 x 12288 15.3 / 14.4.
+constexpr int kFewRows = 32;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -143,7 +146,9 @@ int launch_i8_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorM
 // Pair or one-SM kernel. A k block of either takes an SM its 32 KB at the rate
 // it takes bytes from L2, 0.30 us, for a 128 x 256 share of a pair tile or
 // for a 128 x 128 tile (whose missing rows cost nothing); what counts is the
-// number of rounds.
+// number of rounds. Pair / one-SM, us: 256 x 4096 x 12288 18.3 / 23.8,
+// 512 x 4096 x 4096 16.1 / 12.2, 1024 x 4096 x 4096 17.2 / 22.7,
+// 1024 x 640 x 2048 7.9 / 6.4.
 bool pair_is_faster(int64_t rows, int64_t n) {
   const int sms = sm_count();
   const int64_t pair_tiles = ((rows + 255) / 256) * ((n + 255) / 256), tiles = ((rows + 127) / 128) * ((n + 127) / 128);
@@ -238,9 +243,9 @@ int linear_w8a8(const nd_linear_w8a8_args& a, cudaStream_t stream) {
 
   CUtensorMap ta, tb, tc;
   // More tiles of 128 weight rows than SMs: half the stages, so that two CTAs
-  // share an SM and one's loads run under the other's start and end. That also
-  // takes 33 to 64 rows (otherwise the 128 x 128 tiles' vector epilogue is the
-  // faster one).
+  // share an SM and one's loads run under the other's start and end
+  // (16 x 4096 x 24576 SwiGLU 26.5 -> 20.1 us). That also takes 33 to 64 rows
+  // (48 x 1280 x 24576 10.2 us against 15.6 in 128 x 128 tiles).
   const bool two = (gated ? a.out_features / 64 : (n_all + 127) / 128) > sm_count();
   if (a.rows <= kFewRows || (two && a.rows <= 2 * kFewRows)) {
     const int nt = a.rows <= 16 ? 16 : a.rows <= 32 ? 32 : 64;

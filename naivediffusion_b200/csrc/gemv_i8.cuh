@@ -4,15 +4,19 @@
 //
 // A warp takes two weight rows (the two factors' rows of one output for the
 // gated epilogues): lane l reads 16-byte groups l, l + 32, .. of both rows,
-// four groups of each in flight, against the same groups of x, which stay in
-// L1. One warp per pair of rows and one wave of blocks, so every load of the
-// weights is in flight early.
+// kGroups of each in flight, against the same groups of x, which stay in L1.
+// One warp per pair of rows and about one wave of blocks, so every load of the
+// weights is in flight early: 1 x 4096 x 12288 9.5 us (5.3 TB/s). Two rows of x
+// take two groups and 48 warps per SM (10.2 us against 12.4 with four groups);
+// one, three and four rows lose by that (4 x 4096 x 12288 12.9 against 18.4).
 #pragma once
 
 #include "gemm_i8_sm100.cuh"
 
 namespace nd {
 
+// At four rows against gemm_i8_few_kernel, us: 1024 x 1024 2.5 / 5.4, 4096 x 12288
+// 12.9 / 12.9; a fifth row of x would double the loads from L1 per weight.
 constexpr int kGemvI8Rows = 4;
 constexpr int kGemvI8Threads = 128;
 
@@ -55,7 +59,8 @@ __device__ __forceinline__ float load_16bit(const void* p, long long i, int f16)
 }
 
 template <int MR>
-__global__ void __launch_bounds__(kGemvI8Threads) gemv_i8_kernel(const I8GemvArgs args) {
+__global__ void __launch_bounds__(kGemvI8Threads, MR == 2 ? 12 : 1) gemv_i8_kernel(const I8GemvArgs args) {
+  constexpr int kGroups = MR == 2 ? 2 : 4;
   griddep_launch();
   griddep_wait();
   const I8GemmArgs& a = args.g;
@@ -73,10 +78,10 @@ __global__ void __launch_bounds__(kGemvI8Threads) gemv_i8_kernel(const I8GemvArg
 #pragma unroll
   for (int m = 0; m < MR; ++m) acc[m][0] = acc[m][1] = 0;
 
-  for (int c0 = lane; c0 < groups; c0 += 128) {
-    uint4 p[4], q[4];
+  for (int c0 = lane; c0 < groups; c0 += 32 * kGroups) {
+    uint4 p[kGroups], q[kGroups];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kGroups; ++u) {
       const int c = c0 + 32 * u;
       p[u] = q[u] = make_uint4(0u, 0u, 0u, 0u);
       if (c < groups) {
@@ -85,7 +90,7 @@ __global__ void __launch_bounds__(kGemvI8Threads) gemv_i8_kernel(const I8GemvArg
       }
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kGroups; ++u) {
       const int c = c0 + 32 * u;
       if (c < groups) {
 #pragma unroll

@@ -11,7 +11,9 @@
 // at 4352 x 12288: values of exactly half the peak make one in most rows.
 //
 // Bound by HBM: the row is read once, stays in registers while its peak is
-// found, and one byte per value is written.
+// found, and one byte per value is written. 4352 x 12288 bf16 30 us (5.4 TB/s,
+// 82 % of the copy rate), 8192 x 8192 bf16 34 us (90 %); rows that are no
+// multiple of 8 values go one value at a time (1001 x 5121 fp32 8.3 us, 47 %).
 #include <algorithm>
 #include <climits>
 
@@ -172,7 +174,8 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
 // T threads per row (a warp for narrow rows, four rows to a block), V x VEC
 // values per thread in registers, the rest of a longer row read twice.
 // 1536 threads per SM (40 registers; fp32 vectors take 64) keep enough rows in
-// flight.
+// flight: with fp32 values in registers and 1024 threads 4352 x 12288 bf16 took
+// 52 us, and 32768 x 640 with a block per row 35 us where four warps take 14.
 template <int TYPE, int VEC, int V, int T>
 __global__ void __launch_bounds__(T < 128 ? 128 : T, (TYPE == ND_F32 && VEC == 8 ? 1024 : 1536) / (T < 128 ? 128 : T))
     quantize_rows_kernel(const void* x, long long ldx, int rows, int width, int8_t* q, long long ldq, float* scale) {

@@ -14,7 +14,8 @@
 // Bound by HBM: every element of x and branch is read once, x' and y are
 // written once; the row stays in registers between its (up to five) row-wide
 // reductions. Variances are centred second moments over the registers, in
-// fp32.
+// fp32. 4352 x 4096 (bf16 branch and y) 39 us, 5.5 TB/s, 83 % of the copy rate;
+// 8192 x 2048 to int8 34 us, 82 %; 4000 x 3001 41 us, 54 %.
 #include <algorithm>
 #include <climits>
 
