@@ -549,8 +549,16 @@ int dequantize(const int8_t* q, const void* scales, int scale_dtype, int64_t qua
   if (out_dtype != ND_BF16 && out_dtype != ND_F16) return fail(ND_ERR_INVALID, "dequantize: out_dtype");
   const int64_t group = quant_group > 0 ? quant_group : cols;
   if (cols % group) return fail(ND_ERR_INVALID, "dequantize: quant_group must divide cols");
-  const bool by16 = cols % 16 == 0 && group % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 &&
-                    reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  const bool aligned = reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  const bool by16 = aligned && cols % 16 == 0 && group % 16 == 0;
+  const int64_t runs = (rows * cols + 16 * 256 - 1) / (16 * 256);
+  if (aligned && !by16 && group == cols && cols >= 16 && runs <= INT_MAX) {
+    dequant_rows_kernel<<<static_cast<unsigned>(runs), 256, 0, stream>>>(q, scales, scale_dtype == ND_F16, rows * cols,
+                                                                         static_cast<int>(cols), static_cast<uint16_t*>(out),
+                                                                         out_dtype == ND_F16);
+    ND_CUDA(cudaGetLastError());
+    return ND_OK;
+  }
   const int64_t per_row = (cols + (by16 ? 16 * 128 : 128) - 1) / (by16 ? 16 * 128 : 128);  // blocks to cover a row at once
   const int64_t most = sm_count() * 16LL;
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>(rows, most)),

@@ -96,6 +96,7 @@ __device__ __forceinline__ void few_direct(const I8FewArgs& args, uint32_t tbase
         const float f = a.epi == kEpiGeGlu ? first * i8_gelu_erf(splat(second)).x : i8_silu(splat(first)).x * second;
         if (live && m < a.M) few_store(args, m, col, f);
       }
+      __syncwarp();
       continue;
     }
     switch (a.epi) {
@@ -123,10 +124,11 @@ __device__ __forceinline__ void few_direct(const I8FewArgs& args, uint32_t tbase
       default:
         break;
     }
-    if (!live) continue;
     const int n = a.M - c;  // of these 16 tokens, the first n exist
     const long long o = c * args.ld + col;
-    if (a.epi == kEpiResidualGate || a.epi == kEpiResidualAdd || a.epi == kEpiStoreF32) {
+    if (!live) {
+      // This lane's column is past the output's.
+    } else if (a.epi == kEpiResidualGate || a.epi == kEpiResidualAdd || a.epi == kEpiStoreF32) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         if (i < n) few_store(args, c + i, col, v[i]);
@@ -141,6 +143,7 @@ __device__ __forceinline__ void few_direct(const I8FewArgs& args, uint32_t tbase
       for (int i = 0; i < 16; ++i)
         if (i < n) y[i * args.ld] = __float2bfloat16_rn(v[i]);
     }
+    __syncwarp();  // the next columns are loaded by the whole warp
   }
 }
 

@@ -398,11 +398,59 @@ __global__ void __launch_bounds__(kW8Threads, 1)
 // Standalone dequantization, the same arithmetic as the converters:
 // w[n, k] = bf16/f16(float(q[n, k]) * scale(n, k)). For the bit-exact check
 // against the oracle and for callers that want the widened weight.
+// 16 values (16-byte aligned in and out): the first `n` times s, the others
+// times t.
+__device__ __forceinline__ void dequant16(const int8_t* q, uint16_t* out, float s, float t, int n, int out_f16) {
+  const uint4 p = __ldg(reinterpret_cast<const uint4*>(q));
+  const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+  uint32_t h[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float f[4];
+    i8x4_to_f32(w[i], f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] *= 4 * i + j < n ? s : t;
+    h[2 * i] = out_f16 ? pack_f16(f[0], f[1]) : pack_bf16(f[0], f[1]);
+    h[2 * i + 1] = out_f16 ? pack_f16(f[2], f[3]) : pack_bf16(f[2], f[3]);
+  }
+  uint4* o = reinterpret_cast<uint4*>(out);
+  o[0] = make_uint4(h[0], h[1], h[2], h[3]);
+  o[1] = make_uint4(h[4], h[5], h[6], h[7]);
+}
+
+// One scale per row, rows of any width from 16 on: the matrix as one run of
+// values, 16 per thread, which lie in one row or two. The last total % 16 are
+// left to the last thread.
+__global__ void __launch_bounds__(256) dequant_rows_kernel(const int8_t* __restrict__ q, const void* __restrict__ scales,
+                                                           int scale_f16, long long total, int cols,
+                                                           uint16_t* __restrict__ out, int out_f16) {
+  auto scale = [&](long long r) {
+    return scale_f16 ? __half2float(static_cast<const __half*>(scales)[r]) : static_cast<const float*>(scales)[r];
+  };
+  const long long at = (blockIdx.x * 256LL + threadIdx.x) * 16;
+  if (at >= total) return;
+  const long long r = at >> 32 ? at / cols : static_cast<long long>(static_cast<uint32_t>(at) / static_cast<uint32_t>(cols));
+  const long long left = (r + 1) * cols - at;  // values to the end of the row
+  const int n = static_cast<int>(left < 16 ? left : 16);
+  const float s = scale(r);
+  if (at + 16 <= total) {
+    dequant16(q + at, out + at, s, n < 16 ? scale(r + 1) : s, n, out_f16);
+    return;
+  }
+  for (int i = 0; at + i < total; ++i) {
+    float f[4];
+    i8x4_to_f32(static_cast<uint32_t>(static_cast<uint8_t>(q[at + i])), f);
+    const float v = f[0] * (i < n ? s : scale(r + 1));
+    out[at + i] = static_cast<uint16_t>(out_f16 ? pack_f16(v, 0.f) : pack_bf16(v, 0.f));
+  }
+}
+
 // Blocks of 128 threads walk rows (blockIdx.x, + gridDim.x, ..) and a share of
 // the columns (blockIdx.y), VEC values per thread: 16 (one 16-byte load, two
 // 16-byte stores, one scale) where a group, the row and the pointers allow it,
 // else one. Bound by HBM: 8192 x 2048 with one scale per row takes 11 us, where
-// one value per thread with a division for its row took 58.
+// one value per thread with a division for its row took 58. Rows of any width
+// with one scale each: dequant_rows_kernel.
 template <int VEC>
 __global__ void __launch_bounds__(128) dequant_w8_kernel(const int8_t* __restrict__ q, const void* __restrict__ scales,
                                                          int scale_f16, int group, int scale_cols, long long rows, int cols,
@@ -414,19 +462,7 @@ __global__ void __launch_bounds__(128) dequant_w8_kernel(const int8_t* __restric
       const long long si = r * scale_cols + (scale_cols > 1 ? c / group : 0);
       const float s = scale_f16 ? __half2float(static_cast<const __half*>(scales)[si]) : static_cast<const float*>(scales)[si];
       if constexpr (VEC == 16) {
-        const uint4 p = __ldg(reinterpret_cast<const uint4*>(qr + c));
-        const uint32_t w[4] = {p.x, p.y, p.z, p.w};
-        uint32_t h[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float f[4];
-          i8x4_to_f32(w[i], f);
-          h[2 * i] = out_f16 ? pack_f16(f[0] * s, f[1] * s) : pack_bf16(f[0] * s, f[1] * s);
-          h[2 * i + 1] = out_f16 ? pack_f16(f[2] * s, f[3] * s) : pack_bf16(f[2] * s, f[3] * s);
-        }
-        uint4* o = reinterpret_cast<uint4*>(orow + c);
-        o[0] = make_uint4(h[0], h[1], h[2], h[3]);
-        o[1] = make_uint4(h[4], h[5], h[6], h[7]);
+        dequant16(qr + c, orow + c, s, s, 16, out_f16);
       } else {
         float f[4];
         i8x4_to_f32(static_cast<uint32_t>(static_cast<uint8_t>(qr[c])), f);  // byte 0 is q; the zero bytes are unused

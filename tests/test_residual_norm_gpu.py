@@ -246,7 +246,8 @@ def test_quantize_rows_special_rows_and_strides(cuda):
         assert torch.equal(torch.isnan(scale), torch.isnan(ws)) and torch.equal(scale.nan_to_num(9), ws.nan_to_num(9))
 
 
-@pytest.mark.parametrize("rows,cols", [(1, 1), (77, 2048), (3000, 640), (1001, 5121), (9, 40000), (5000, 48)])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (77, 2048), (3000, 640), (1001, 5121), (9, 40000), (5000, 48), (700, 17),
+                                       (33, 21), (3, 5), (1, 16), (257, 1155)])
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_values_of_int8_rows(cuda, rows, cols, dtype):
     """dequantize gives back what a quantized row stands for, rounded once: within half a step of x and of dtype."""
