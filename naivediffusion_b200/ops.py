@@ -244,10 +244,6 @@ def _packer(args):
 _pack_residual_norm, _pack_linear_w8a8 = _packer(ResidualNormArgs), _packer(LinearW8A8Args)
 
 
-def _addr(t: torch.Tensor | None) -> int:
-    return 0 if t is None else t.data_ptr()
-
-
 def _round_up(n: int, multiple: int) -> int:
     return (n + multiple - 1) // multiple * multiple
 
@@ -256,13 +252,23 @@ def _matrix(what: str, t: torch.Tensor, dtypes, device, multiple: int = 1) -> tu
     """Rows, columns and row stride of a matrix with unit column stride. A single row's stride is never used and may
     be anything: the next multiple of `multiple` then."""
     if t.dtype in dtypes and t.device == device:
-        shape, stride = t.shape, t.stride()
-        if len(shape) == 2:
-            rows, cols = shape
+        stride = t.stride()
+        if len(stride) == 2:
+            rows, cols = t.shape
             if stride[1] == 1 or cols == 1:
                 return rows, cols, stride[0] if rows > 1 else _round_up(cols, multiple)
     raise ValueError(f"{what} must be a 2-D {'/'.join(str(d) for d in dtypes)} tensor with unit column stride on "
                      f"{device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+
+
+def _vector(what: str, t: torch.Tensor | None, n: int, device) -> int:
+    """The address of a vector that holds n values (0 for None)."""
+    if t is None:
+        return 0
+    if t.dtype is _F32 and t.device == device and t.numel() >= n and t.is_contiguous():
+        return t.data_ptr()
+    _check_vec(what, t, n, device)
+    return t.data_ptr()
 
 
 def _output(what: str, t: torch.Tensor, rows: int, cols: int, dtypes, device, multiple: int = 1) -> int:
@@ -294,7 +300,11 @@ def _launch(what: str, device, fn, *args) -> None:
         check(code)
 
 
-_FP32, _INT8, _HALVES = (torch.float32,), (torch.int8,), (torch.bfloat16, torch.float16)
+_F32, _I8 = torch.float32, torch.int8
+_RESIDUAL_EPI = (_lib.ND_EPI_RESIDUAL_GATE, _lib.ND_EPI_RESIDUAL_ADD, _lib.ND_EPI_STORE_F32)
+_GATED_EPI = (_lib.ND_EPI_SWIGLU, _lib.ND_EPI_GEGLU)
+_VECTORS = ("residual_norm: gate", "residual_norm: scale", "residual_norm: shift")
+_FP32, _INT8, _HALVES = (_F32,), (_I8,), (torch.bfloat16, torch.float16)
 
 
 def residual_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *, x_out: torch.Tensor | None = None,
@@ -316,58 +326,55 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *, x_out:
     """
     device = x.device
     rows, width, ldx = _matrix("residual_norm: x", x, _FP32, device)
-    ldb = b_type = ldo = 0
+    x_ptr = x.data_ptr()
+    b_ptr = ldb = b_type = 0
     if branch is not None:
         have, wide, ldb = _matrix("residual_norm: branch", branch, _FLOATS, device)
         if have != rows or wide != width:
             raise ValueError(f"residual_norm: branch must be [{rows}, {width}], got {tuple(branch.shape)}")
-        b_type = _DT[branch.dtype]
-    if post_weight is not None:
-        _check_vec("residual_norm: post_weight", post_weight, width, device)
-    if pre_weight is not None:
-        _check_vec("residual_norm: pre_weight", pre_weight, width, device)
-    vecs, vec_stride = 0, width
-    for name, t in (("gate", gate), ("scale", scale), ("shift", shift)):
+        b_ptr, b_type = branch.data_ptr(), _DT[branch.dtype]
+    post_ptr = _vector("residual_norm: post_weight", post_weight, width, device)
+    pre_ptr = _vector("residual_norm: pre_weight", pre_weight, width, device)
+    vecs, vec_stride, ptrs = 0, width, [0, 0, 0]
+    for i, t in enumerate((gate, scale, shift)):
         if t is None:
             continue
-        if t.dim() == 1:
-            t = t[None]
-        sets, wide, stride = _matrix(f"residual_norm: {name}", t, _FP32, device)
+        name = _VECTORS[i]
+        sets, wide, stride = _matrix(name, t if t.dim() != 1 else t[None], _FP32, device)
         if vecs == 0:
             vecs, vec_stride = sets, stride
         if wide != width or sets != vecs or stride != vec_stride:
-            raise ValueError(f"residual_norm: {name} must be [{width}] or [vecs, {width}] with the others' number of "
-                             f"sets and row stride, got {tuple(t.shape)} with stride {stride}")
+            raise ValueError(f"{name} must be [{width}] or [vecs, {width}] with the others' number of sets and row stride, "
+                             f"got {tuple(t.shape)} with stride {stride}")
+        ptrs[i] = t.data_ptr()
     if vecs > 1 and rows_per_vec <= 0:
         raise ValueError("residual_norm: several vector sets need rows_per_vec")
-    x_new = x
+    x_new, xo_ptr, ldo = x, 0, 0
     if x_out is not None:
         ldo = _output("residual_norm: x_out", x_out, rows, width, _FP32, device)
-        x_new = x_out
+        x_new, xo_ptr = x_out, x_out.data_ptr()
     elif branch is not None or residual_scale != 1.0:
-        x_out, ldo = x, ldx
-    ldy = y_type = 0
+        xo_ptr, ldo = x_ptr, ldx
+    y_ptr = ldy = y_type = q_ptr = 0
     if out is not None:
-        ldy = _output("residual_norm: out", out, rows, width, (*_FLOATS, torch.int8), device)
+        ldy = _output("residual_norm: out", out, rows, width, (*_FLOATS, _I8), device)
         out_dtype = out.dtype
     elif out_dtype is not None:
         if out_dtype not in _DT8:
             raise ValueError(f"residual_norm: out_dtype must be a float type, torch.int8 or None, got {out_dtype}")
-        out, ldy = _padded(rows, width, 16 if out_dtype is torch.int8 else 1, device, out_dtype)
-    int8 = out_dtype is torch.int8
+        out, ldy = _padded(rows, width, 16 if out_dtype is _I8 else 1, device, out_dtype)
+    int8 = out_dtype is _I8
     if int8:
         if out_scale is None:
-            out_scale = torch.empty(rows, device=device, dtype=torch.float32)
-        else:
-            _check_vec("residual_norm: out_scale", out_scale, rows, device)
+            out_scale = torch.empty(rows, device=device, dtype=_F32)
+        q_ptr = _vector("residual_norm: out_scale", out_scale, rows, device)
     elif out_scale is not None:
         raise ValueError("residual_norm: out_scale goes with an int8 output")
     if out is not None:
-        y_type = _DT8[out_dtype]
-    a = _pack_residual_norm(rows, width, x.data_ptr(), ldx, _addr(x_out), ldo, _addr(branch), ldb, b_type, post_norm,
-                            _addr(post_weight), _addr(gate), residual_scale, pre_norm, _addr(pre_weight), _addr(scale),
-                            _addr(shift), vecs or 1, vec_stride, rows_per_vec, 1 if plus_one else 0, eps, _addr(out), ldy,
-                            y_type, _addr(out_scale))
+        y_ptr, y_type = out.data_ptr(), _DT8[out_dtype]
+    a = _pack_residual_norm(rows, width, x_ptr, ldx, xo_ptr, ldo, b_ptr, ldb, b_type, post_norm, post_ptr, ptrs[0],
+                            residual_scale, pre_norm, pre_ptr, ptrs[1], ptrs[2], vecs or 1, vec_stride, rows_per_vec,
+                            1 if plus_one else 0, eps, y_ptr, ldy, y_type, q_ptr)
     _launch("residual_norm", device, lib().nd_op_residual_norm, a)
     return (x_new, out, out_scale) if int8 else (x_new, out)
 
@@ -384,11 +391,9 @@ def quantize_rows(x: torch.Tensor, *, out: torch.Tensor | None = None,
     else:
         ldq = _output("quantize_rows: out", out, rows, cols, _INT8, device, 16)
     if scale is None:
-        scale = torch.empty(rows, device=device, dtype=torch.float32)
-    else:
-        _check_vec("quantize_rows: scale", scale, rows, device)
+        scale = torch.empty(rows, device=device, dtype=_F32)
     _launch("quantize_rows", device, lib().nd_op_quantize_rows, x.data_ptr(), _DT[x.dtype], rows, cols, ldx,
-            out.data_ptr(), ldq, scale.data_ptr())
+            out.data_ptr(), ldq, _vector("quantize_rows: scale", scale, rows, device))
     return out, scale
 
 
@@ -412,28 +417,25 @@ def linear_w8a8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, w_
     w_rows, w_cols, ldw = _matrix("linear_w8a8: weight", weight, _INT8, device, 16)
     split = group_split is not None and group_split < rows
     groups = 2 if split and not shared_weights else 1
-    gated = epilogue in (_lib.ND_EPI_SWIGLU, _lib.ND_EPI_GEGLU)
+    gated = epilogue in _GATED_EPI
     each = w_rows // groups
     n = each // 2 if gated else each
     if w_cols != k or each * groups != w_rows or (gated and each % 2):
         raise ValueError(f"linear_w8a8: weight must be [{groups} * {'2 * ' if gated else ''}out, {k}], got {tuple(weight.shape)}")
-    _check_vec("linear_w8a8: x_scale", x_scale, rows, device)
-    _check_vec("linear_w8a8: w_scale", w_scale, w_rows, device)
-    if bias is not None:
-        _check_vec("linear_w8a8: bias", bias, (2 if split else 1) * each, device)
-    if gate is not None:
-        _check_vec("linear_w8a8: gate", gate, (2 if split else 1) * n, device)
-    ldy = ldr = lda = 0
-    if epilogue in (_lib.ND_EPI_RESIDUAL_GATE, _lib.ND_EPI_RESIDUAL_ADD, _lib.ND_EPI_STORE_F32):
+    sx_ptr = _vector("linear_w8a8: x_scale", x_scale, rows, device)
+    sw_ptr = _vector("linear_w8a8: w_scale", w_scale, w_rows, device)
+    bias_ptr = _vector("linear_w8a8: bias", bias, (2 if split else 1) * each, device)
+    gate_ptr = _vector("linear_w8a8: gate", gate, (2 if split else 1) * n, device)
+    y_ptr = ldy = r_ptr = ldr = a_ptr = lda = 0
+    if epilogue in _RESIDUAL_EPI:
         if residual is not None:
             ldr = _output("linear_w8a8: residual", residual, rows, n, _FP32, device, 4)
         elif epilogue == _lib.ND_EPI_STORE_F32:
-            residual, ldr = _padded(rows, n, 4, device, torch.float32)
+            residual, ldr = _padded(rows, n, 4, device, _F32)
         else:
             raise ValueError("linear_w8a8: this epilogue adds to residual, and none is given")
-        out, out_dtype = None, torch.bfloat16
+        result, r_ptr, out_dtype = residual, residual.data_ptr(), torch.bfloat16
     else:
-        residual = None
         if out is not None:
             ldy = _output("linear_w8a8: out", out, rows, n, _HALVES, device, 8)
             out_dtype = out.dtype
@@ -441,14 +443,15 @@ def linear_w8a8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, w_
             out, ldy = _padded(rows, n, 8, device, out_dtype)
         else:
             raise ValueError(f"linear_w8a8: out_dtype must be float16 or bfloat16 (STORE_F32 for fp32), got {out_dtype}")
+        result, y_ptr = out, out.data_ptr()
     if addend is not None:
         lda = _output("linear_w8a8: addend", addend, rows, n, (out_dtype,), device)
-    a = _pack_linear_w8a8(_DT[out_dtype], epilogue, rows, k, n, x.data_ptr(), ldx, x_scale.data_ptr(), weight.data_ptr(),
-                          ldw, w_scale.data_ptr(), _addr(bias), rows if group_split is None else group_split,
-                          1 if shared_weights else 0, _addr(out), ldy, _addr(residual), ldr, _addr(gate), 0,
-                          _addr(addend), lda)
+        a_ptr = addend.data_ptr()
+    a = _pack_linear_w8a8(_DT[out_dtype], epilogue, rows, k, n, x.data_ptr(), ldx, sx_ptr, weight.data_ptr(), ldw, sw_ptr,
+                          bias_ptr, rows if group_split is None else group_split, 1 if shared_weights else 0, y_ptr, ldy,
+                          r_ptr, ldr, gate_ptr, 0, a_ptr, lda)
     _launch("linear_w8a8", device, lib().nd_op_linear_w8a8, a)
-    return out if residual is None else residual
+    return result
 
 
 def rmsnorm(x: torch.Tensor, weight: torch.Tensor | None, *, out_dtype=None, plus_one=False,
