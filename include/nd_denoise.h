@@ -513,7 +513,10 @@ ND_API int nd_op_quantize_rows(const void* x, int dtype, int64_t rows, int64_t c
  * weights and multiplies in 16 bits; this is the 8-bit product itself.
  * Row groups (group_split, shared_weights), the epilogues and their operands
  * are nd_linear_args'; QK_NORM_ROPE is not offered (nd_op_head_norm_rope runs
- * after a STORE). */
+ * after a STORE). Repeated calls give the same bits. There is no workspace:
+ * calls on different streams, and captured ones, share nothing. The first call
+ * on a device (this one's or nd_op_residual_norm's) allocates the library's
+ * status word: make it before a stream capture. */
 typedef struct nd_linear_w8a8_args {
   int dtype;            /* ND_BF16 or ND_F16: y and addend */
   int epilogue;         /* ND_EPI_* except QK_NORM_ROPE */
@@ -534,7 +537,7 @@ typedef struct nd_linear_w8a8_args {
   int64_t ldr;
   const float* gate;    /* [groups][gate_stride] (RESIDUAL_GATE) */
   int64_t gate_stride;  /* 0: out_features */
-  const void* addend;   /* ADD_STORE: [rows, ld_add], dtype like y */
+  const void* addend;   /* ADD_STORE: [rows, ld_add], dtype like y; may be y itself */
   int64_t ld_add;
 } nd_linear_w8a8_args;
 

@@ -249,6 +249,29 @@ def test_streams_and_graphs(cuda, m):
     assert torch.equal(y, b.to(BF16).expand(m, -1))
 
 
+@pytest.mark.parametrize("m", [1, 20, 100, 300, 1200])
+def test_the_addend_may_be_the_output(cuda, m):
+    from naivediffusion_b200 import ops
+    n, k = 1000, 640
+    g, x, sx, w, sw, b = _case(m, n, k, m + 5)
+    base = torch.randn(m, n, generator=g, device="cuda").to(BF16)
+    want = ops.linear_w8a8(x, sx, w, sw, b, epilogue=EPI["add_store"], addend=base)
+    y = base.clone()
+    got = ops.linear_w8a8(x, sx, w, sw, b, epilogue=EPI["add_store"], addend=y, out=y)
+    ops.sync()
+    assert got is y and torch.equal(y, want)
+
+
+@pytest.mark.parametrize("m", [1, 2, 20, 60, 1100])
+def test_every_kernel_repeats_itself(cuda, m):
+    """The same call twice gives the same bits: integer sums, and no order that varies."""
+    from naivediffusion_b200 import ops
+    _, x, sx, w, sw, b = _case(m, 768, 9000, m)
+    y = [ops.linear_w8a8(x, sx, w, sw, b, epilogue=EPI["gelu_erf"]) for _ in range(4)]
+    ops.sync()
+    assert all(torch.equal(t, y[0]) for t in y)
+
+
 def test_a_block_of_them(cuda):
     """A transformer block's MLP as it runs on 8 bits: norm to int8, gate and up product, its rows to int8, down
     product, gated residual and the next norm. Each step against 64 bits on what the step before stored, and the

@@ -289,3 +289,35 @@ def test_streams_and_graphs(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert got[1].eq(0).all() and q[1].eq(0).all()
+
+
+@pytest.mark.parametrize("rows,width", [(5000, 2048), (3000, 2047)])
+def test_many_rows_in_place_on_two_streams_and_captured(cuda, rows, width):
+    """Persistent blocks of two calls at once share nothing; a captured in-place call goes on from what it left."""
+    from naivediffusion_b200 import ops
+    cases = [_inputs(rows, width, BF16, 2, seed) for seed in (1, 2)]
+    kw = [dict(gate=v[:, 0], scale=v[:, 1], shift=v[:, 2], rows_per_vec=rows // 2, post_norm=RMS, out_dtype=BF16) for _, _, v, _, _ in cases]
+    want = []
+    for (x, b, _, _, _), k in zip(cases, kw):
+        x = x.clone()
+        want.append([[t.clone() for t in ops.residual_norm(x, b, **k)] for _ in range(3)])
+    torch.cuda.synchronize()
+    xs = [c[0].clone() for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for _ in range(3):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append([t.clone() for t in ops.residual_norm(xs[i], cases[i][1], **kw[i])])
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(p, q) for a, b in zip(w, g) for p, q in zip(a, b))
+    x = cases[0][0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        new, y = ops.residual_norm(x, cases[0][1], **kw[0])
+    x.copy_(cases[0][0])
+    for step in range(3):
+        graph.replay()
+        ops.sync()
+        assert new is x and torch.equal(x, want[0][step][0]) and torch.equal(y, want[0][step][1])
