@@ -13,7 +13,9 @@
 // Bound by HBM: the row is read once, stays in registers while its peak is
 // found, and one byte per value is written. 4352 x 12288 bf16 30 us (5.4 TB/s,
 // 82 % of the copy rate), 8192 x 8192 bf16 34 us (90 %); rows that are no
-// multiple of 8 values go one value at a time (1001 x 5121 fp32 8.3 us, 47 %).
+// multiple of 8 values are read a value at a time, four neighbours per thread
+// (1001 x 5121 fp32 7.6 us, 51 %; 4000 x 9001 bf16 47 us where one value per
+// thread and store took 54).
 #include <algorithm>
 #include <climits>
 
@@ -32,14 +34,16 @@ constexpr float kNearHalf = 0.49997f;
 // A thread's share of a row as it lies in memory: VEC values of one type. The
 // 16-bit types stay packed until they are quantized (half the registers, so
 // twice the rows in flight), and |x| is compared as integers: bit patterns of
-// one sign order like the values, with NaN above infinity.
+// one sign order like the values, with NaN above infinity. VEC = 8: vector loads
+// (aligned rows); 4: single loads of four neighbours (rows of any width and
+// alignment, whose int8 rows still take 4-byte stores), of which `n` exist; 1.
 template <int TYPE, int VEC>
 struct Raw;
 template <>
 struct Raw<ND_F32, 8> {
   float4 w[2];
   __device__ __forceinline__ void clear() { w[0] = w[1] = make_float4(0.f, 0.f, 0.f, 0.f); }
-  __device__ __forceinline__ void load(const void* p, long long i) {
+  __device__ __forceinline__ void load(const void* p, long long i, int) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
       asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0,%1,%2,%3}, [%4];"
@@ -62,9 +66,26 @@ template <>
 struct Raw<ND_F32, 1> {
   float w;
   __device__ __forceinline__ void clear() { w = 0.f; }
-  __device__ __forceinline__ void load(const void* p, long long i) { w = __ldg(static_cast<const float*>(p) + i); }
+  __device__ __forceinline__ void load(const void* p, long long i, int) { w = __ldg(static_cast<const float*>(p) + i); }
   __device__ __forceinline__ void peak(uint32_t& m) const { m = max(m, abs_bits(w)); }
   __device__ __forceinline__ void values(float (&f)[1]) const { f[0] = w; }
+};
+template <>
+struct Raw<ND_F32, 4> {
+  float w[4];
+  __device__ __forceinline__ void clear() { w[0] = w[1] = w[2] = w[3] = 0.f; }
+  __device__ __forceinline__ void load(const void* p, long long i, int n) {
+    const float* f = static_cast<const float*>(p) + i;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = j < n ? __ldg(f + j) : 0.f;
+  }
+  __device__ __forceinline__ void peak(uint32_t& m) const {
+    m = max(max(m, max(abs_bits(w[0]), abs_bits(w[1]))), max(abs_bits(w[2]), abs_bits(w[3])));
+  }
+  __device__ __forceinline__ void values(float (&f)[4]) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = w[j];
+  }
 };
 template <int TYPE>
 __device__ __forceinline__ float2 halves(uint32_t w) {
@@ -75,7 +96,7 @@ template <int TYPE>
 struct Raw<TYPE, 8> {
   uint4 w;
   __device__ __forceinline__ void clear() { w = make_uint4(0u, 0u, 0u, 0u); }
-  __device__ __forceinline__ void load(const void* p, long long i) {
+  __device__ __forceinline__ void load(const void* p, long long i, int) {
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
                  : "l"(static_cast<const uint16_t*>(p) + i));
@@ -95,10 +116,30 @@ struct Raw<TYPE, 8> {
   }
 };
 template <int TYPE>
+struct Raw<TYPE, 4> {
+  uint32_t w[2];
+  __device__ __forceinline__ void clear() { w[0] = w[1] = 0u; }
+  __device__ __forceinline__ void load(const void* p, long long i, int n) {
+    const uint16_t* h = static_cast<const uint16_t*>(p) + i;
+    uint32_t t[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) t[j] = j < n ? __ldg(h + j) : 0u;
+    w[0] = __byte_perm(t[0], t[1], 0x5410);
+    w[1] = __byte_perm(t[2], t[3], 0x5410);
+  }
+  __device__ __forceinline__ void peak(uint32_t& m) const {  // two 16-bit maxima
+    m = __vmaxu2(m, __vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu));
+  }
+  __device__ __forceinline__ void values(float (&f)[4]) const {
+    const float2 a = halves<TYPE>(w[0]), b = halves<TYPE>(w[1]);
+    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
+  }
+};
+template <int TYPE>
 struct Raw<TYPE, 1> {
   uint16_t w;
   __device__ __forceinline__ void clear() { w = 0; }
-  __device__ __forceinline__ void load(const void* p, long long i) { w = __ldg(static_cast<const uint16_t*>(p) + i); }
+  __device__ __forceinline__ void load(const void* p, long long i, int) { w = __ldg(static_cast<const uint16_t*>(p) + i); }
   __device__ __forceinline__ void peak(uint32_t& m) const { m = max(m, static_cast<uint32_t>(w & 0x7fff)); }
   __device__ __forceinline__ void values(float (&f)[1]) const { f[0] = halves<TYPE>(w).x; }
 };
@@ -124,15 +165,15 @@ __device__ __forceinline__ float near_half(float x, float r, float peak) {
   return past > 0.f || (past == 0.f && odd) ? r + way : r;
 }
 
-// VEC values (already multiplied by `shift`'s power of two) to int8.
+// VEC values (already multiplied by `shift`'s power of two) to int8, of which n exist.
 template <int VEC>
-__device__ __forceinline__ void quantize_store(int8_t* q, const float (&f)[VEC], float inverse, float peak) {
+__device__ __forceinline__ void quantize_store(int8_t* q, const float (&f)[VEC], float inverse, float peak, int n) {
   float m[VEC];  // rint(t) + 1.5 * 2^23
   float most = 0.f;
-  if constexpr (VEC == 8) {
+  if constexpr (VEC > 1) {
     const float2 inv2 = make_float2(inverse, inverse), magic2 = make_float2(kRintMagic, kRintMagic);
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) {
+    for (int j = 0; j < VEC; j += 2) {
       const float2 x2 = make_float2(f[j], f[j + 1]);
       const float2 m2 = ffma2(x2, inv2, magic2);
       const float2 r2 = fadd2(magic2, make_float2(-m2.x, -m2.y));
@@ -153,6 +194,13 @@ __device__ __forceinline__ void quantize_store(int8_t* q, const float (&f)[VEC],
     *reinterpret_cast<uint2*>(q) =
         make_uint2(pack_low_bytes(__float_as_uint(m[0]), __float_as_uint(m[1]), __float_as_uint(m[2]), __float_as_uint(m[3])),
                    pack_low_bytes(__float_as_uint(m[4]), __float_as_uint(m[5]), __float_as_uint(m[6]), __float_as_uint(m[7])));
+  } else if constexpr (VEC == 4) {
+    const uint32_t w = pack_low_bytes(__float_as_uint(m[0]), __float_as_uint(m[1]), __float_as_uint(m[2]), __float_as_uint(m[3]));
+    if (n >= 4) {
+      *reinterpret_cast<uint32_t*>(q) = w;
+    } else {
+      for (int j = 0; j < n; ++j) q[j] = static_cast<int8_t>((w >> (8 * j)) & 0xffu);
+    }
   } else {
     *q = static_cast<int8_t>(__float_as_uint(m[0]) & 0xffu);
   }
@@ -193,13 +241,13 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T, (TYPE == ND_F32 && VEC == 8
   for (int i = 0; i < V; ++i) {
     const int c = (t + T * i) * VEC;
     v[i].clear();
-    if (c < width) v[i].load(x, x0 + c);
+    if (c < width) v[i].load(x, x0 + c, width - c);
   }
 #pragma unroll
   for (int i = 0; i < V; ++i) v[i].peak(peak);
   for (int c = (t + T * V) * VEC; c < width; c += T * VEC) {
     Raw<TYPE, VEC> w;
-    w.load(x, x0 + c);
+    w.load(x, x0 + c, width - c);
     w.peak(peak);
   }
   const RowScale s = row_scale(block_max<T>(peak_bits<TYPE>(peak), red));
@@ -208,7 +256,7 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T, (TYPE == ND_F32 && VEC == 8
   if (s.inverse == 0.f) {  // zeros, or infinities and NaN: every q is 0
     const float zero[VEC] = {};
 #pragma unroll 1
-    for (int c = t * VEC; c < width; c += T * VEC) quantize_store<VEC>(out + c, zero, 0.f, 1.f);
+    for (int c = t * VEC; c < width; c += T * VEC) quantize_store<VEC>(out + c, zero, 0.f, 1.f, width - c);
     return;
   }
   // Where 127 / peak or 127 x would leave fp32's range, the row is worked on
@@ -223,7 +271,7 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T, (TYPE == ND_F32 && VEC == 8
 #pragma unroll
       for (int j = 0; j < VEC; ++j) w[j] *= shift;
     }
-    quantize_store<VEC>(out + c, w, inverse, row_peak);
+    quantize_store<VEC>(out + c, w, inverse, row_peak, width - c);
   };
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -232,7 +280,7 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T, (TYPE == ND_F32 && VEC == 8
   }
   for (int c = (t + T * V) * VEC; c < width; c += T * VEC) {
     Raw<TYPE, VEC> w;
-    w.load(x, x0 + c);
+    w.load(x, x0 + c, width - c);
     finish(c, w);
   }
 }
@@ -255,10 +303,13 @@ int launch(const void* x, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, in
     else if (w8 <= 1024) ND_QR(8, 4, 256);
     else if (w8 <= 1536) ND_QR(8, 3, 512);
     else ND_QR(8, 4, 512);
+  } else if (ldq % 4 == 0 && reinterpret_cast<uintptr_t>(q) % 4 == 0) {
+    if (cols <= 512) ND_QR(4, 4, 32);
+    else if (cols <= 2048) ND_QR(4, 4, 128);
+    else if (cols <= 4096) ND_QR(4, 4, 256);
+    else ND_QR(4, 4, 512);
   } else {
-    if (cols <= 256) ND_QR(1, 8, 32);
-    else if (cols <= 2048) ND_QR(1, 8, 256);
-    else if (cols <= 4096) ND_QR(1, 8, 512);
+    if (cols <= 2048) ND_QR(1, 8, 256);
     else ND_QR(1, 12, 512);
   }
 #undef ND_QR

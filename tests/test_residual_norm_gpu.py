@@ -196,7 +196,8 @@ def test_values_far_from_one(cuda):
 
 
 @pytest.mark.parametrize("rows,width", [(1, 1), (1, 77), (77, 2048), (5, 130), (300, 513), (33, 4096), (17, 5121), (3, 12288),
-                                        (2, 20001), (1, 40000)])
+                                        (2, 20001), (1, 40000), (40, 1), (41, 2), (19, 3), (500, 511), (130, 2047), (9, 4095),
+                                        (1200, 8191), (3, 16383)])
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 def test_quantize_rows_is_exact(cuda, rows, width, dtype):
     from naivediffusion_b200 import ops
