@@ -94,13 +94,13 @@ int launch_i8(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& t
 
 // The kernel for few rows: 128 weight rows x NT tokens.
 template <int NT, int STAGES>
-int launch_i8_few(const CUtensorMap& tw, const CUtensorMap& tx, const I8FewArgs& g, cudaStream_t stream) {
+int launch_i8_few(const CUtensorMap& tw, const CUtensorMap& tx, const I8GemmArgs& g, cudaStream_t stream) {
   using L = I8FewSmem<NT, STAGES>;
   static int most[64][kMaxSplits + 1] = {};
   int dev = 0;
   if (int rc = current_device(&dev)) return rc;
-  const int tiles = g.g.half > 0 ? g.g.half / 64 : (g.g.N + 127) / 128;
-  return launch_split(gemm_i8_few_kernel<NT, STAGES>, most[dev & 63], L::kLaunchBytes, tiles, (g.g.K + 127) / 128,
+  const int tiles = g.half > 0 ? g.half / 64 : (g.N + 127) / 128;
+  return launch_split(gemm_i8_few_kernel<NT, STAGES>, most[dev & 63], L::kLaunchBytes, tiles, (g.K + 127) / 128,
                       SplitCost{0.17f, 0.f, 0.25f}, stream, tw, tx, g);
 }
 
@@ -157,16 +157,13 @@ bool pair_is_faster(int64_t rows, int64_t n) {
   return pair_rounds < rounds * (0.5f + 0.5f * real);
 }
 
-int launch_i8_gemv(const nd_linear_w8a8_args& a, const I8GemmArgs& g, int64_t ldw, bool resid, cudaStream_t stream) {
+int launch_i8_gemv(const nd_linear_w8a8_args& a, const I8GemmArgs& g, int64_t ldw, cudaStream_t stream) {
   I8GemvArgs v{};
   v.g = g;
   v.x = a.x;
   v.w = a.weight;
   v.ldx = a.ldx;
   v.ldw = ldw;
-  v.y = a.y;
-  v.residual = a.residual;
-  v.ld = resid ? a.ldr : a.ldy;
   const int warps = g.half > 0 ? g.half : (g.N + 1) / 2;
   const dim3 grid((warps + kGemvI8Threads / 32 - 1) / (kGemvI8Threads / 32));
   switch (g.M) {
@@ -236,10 +233,13 @@ int linear_w8a8(const nd_linear_w8a8_args& a, cudaStream_t stream) {
   g.gate_stride = a.gate_stride > 0 ? a.gate_stride : a.out_features;
   g.addend = a.addend;
   g.ld_add = a.ld_add;
+  g.y = static_cast<uint16_t*>(a.y);
+  g.residual = a.residual;
+  g.ld = resid ? a.ldr : a.ldy;
   g.status = device_status();
   if (!g.status) return fail(ND_ERR_CUDA, "linear_w8a8: no device status word");
 
-  if (a.rows <= kGemvI8Rows) return launch_i8_gemv(a, g, ldw, resid, stream);
+  if (a.rows <= kGemvI8Rows) return launch_i8_gemv(a, g, ldw, stream);
 
   CUtensorMap ta, tb, tc;
   // More tiles of 128 weight rows than SMs: half the stages, so that two CTAs
@@ -253,15 +253,10 @@ int linear_w8a8(const nd_linear_w8a8_args& a, cudaStream_t stream) {
     if (rc) return rc;
     rc = make_tmap_2d(&tb, a.x, 1, a.rows, a.in_features, a.ldx, nt, 128, true);
     if (rc) return rc;
-    I8FewArgs f{};
-    f.g = g;
-    f.g.idesc = make_idesc_i8(128, nt);
-    f.y = a.y;
-    f.residual = a.residual;
-    f.ld = resid ? a.ldr : a.ldy;
-    if (nt == 16) return two ? launch_i8_few<16, 6>(ta, tb, f, stream) : launch_i8_few<16, 12>(ta, tb, f, stream);
-    if (nt == 32) return two ? launch_i8_few<32, 5>(ta, tb, f, stream) : launch_i8_few<32, 11>(ta, tb, f, stream);
-    return launch_i8_few<64, 4>(ta, tb, f, stream);
+    g.idesc = make_idesc_i8(128, nt);
+    if (nt == 16) return two ? launch_i8_few<16, 6>(ta, tb, g, stream) : launch_i8_few<16, 12>(ta, tb, g, stream);
+    if (nt == 32) return two ? launch_i8_few<32, 5>(ta, tb, g, stream) : launch_i8_few<32, 11>(ta, tb, g, stream);
+    return launch_i8_few<64, 4>(ta, tb, g, stream);
   }
   int rc = make_tmap_2d(&ta, a.x, 1, a.rows, a.in_features, a.ldx, 128, 128, true);
   if (rc) return rc;

@@ -34,13 +34,6 @@ struct I8FewSmem {
   static constexpr int kTmemCols = NT < 32 ? 32 : NT;
 };
 
-struct I8FewArgs {
-  I8GemmArgs g;
-  void* y;          // 16-bit output, or
-  float* residual;  // the fp32 epilogues'
-  long long ld;
-};
-
 __device__ __forceinline__ int2 ld_shared_cluster2(uint32_t addr) {
   int2 v;
   asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
@@ -48,19 +41,16 @@ __device__ __forceinline__ int2 ld_shared_cluster2(uint32_t addr) {
 }
 
 // One finished value v (the epilogue's activations are applied) at (m, col).
-__device__ __forceinline__ void few_store(const I8FewArgs& args, int m, int col, float v) {
-  const I8GemmArgs& a = args.g;
-  const long long o = m * args.ld + col;
-  if (a.epi == kEpiStoreF32) args.residual[o] = v;
-  else if (a.epi == kEpiResidualGate || a.epi == kEpiResidualAdd) args.residual[o] += v;
-  else if (a.out_f16) static_cast<__half*>(args.y)[o] = __float2half_rn(v);
-  else static_cast<__nv_bfloat16*>(args.y)[o] = __float2bfloat16_rn(v);
+__device__ __forceinline__ void few_store(const I8GemmArgs& a, int m, int col, float v) {
+  const long long o = m * a.ld + col;
+  if (a.epi == kEpiStoreF32) a.residual[o] = v;
+  else if (a.epi == kEpiResidualGate || a.epi == kEpiResidualAdd) a.residual[o] += v;
+  else a.y[o] = static_cast<uint16_t>(a.out_f16 ? pack_f16(v, 0.f) : pack_bf16(v, 0.f));
 }
 
 // S = 1: this lane's weight row of tile `tile` against every token.
 template <int NT>
-__device__ __forceinline__ void few_direct(const I8FewArgs& args, uint32_t tbase, int tile, int ew, int lane) {
-  const I8GemmArgs& a = args.g;
+__device__ __forceinline__ void few_direct(const I8GemmArgs& a, uint32_t tbase, int tile, int ew, int lane) {
   const bool gated = a.half > 0;
   const int col = gated ? tile * 64 + ew * 16 + (lane & 15) : tile * 128 + ew * 32 + lane;
   const int wrow = gated && lane >= 16 ? a.half + col : col;
@@ -94,7 +84,7 @@ __device__ __forceinline__ void few_direct(const I8FewArgs& args, uint32_t tbase
         const float first = upper ? got : v[i], second = upper ? v[i + 1] : got;
         const int m = c + i + (upper ? 1 : 0);
         const float f = a.epi == kEpiGeGlu ? first * i8_gelu_erf(splat(second)).x : i8_silu(splat(first)).x * second;
-        if (live && m < a.M) few_store(args, m, col, f);
+        if (live && m < a.M) few_store(a, m, col, f);
       }
       __syncwarp();
       continue;
@@ -125,23 +115,23 @@ __device__ __forceinline__ void few_direct(const I8FewArgs& args, uint32_t tbase
         break;
     }
     const int n = a.M - c;  // of these 16 tokens, the first n exist
-    const long long o = c * args.ld + col;
     if (!live) {
       // This lane's column is past the output's.
     } else if (a.epi == kEpiResidualGate || a.epi == kEpiResidualAdd || a.epi == kEpiStoreF32) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (i < n) few_store(args, c + i, col, v[i]);
-    } else if (a.out_f16) {
-      __half* y = static_cast<__half*>(args.y) + o;
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (i < n) y[i * args.ld] = __float2half_rn(v[i]);
+        if (i < n) few_store(a, c + i, col, v[i]);
     } else {
-      __nv_bfloat16* y = static_cast<__nv_bfloat16*>(args.y) + o;
+      uint16_t* y = a.y + c * a.ld + col;
+      if (a.out_f16) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (i < n) y[i * args.ld] = __float2bfloat16_rn(v[i]);
+        for (int i = 0; i < 16; ++i)
+          if (i < n) y[i * a.ld] = static_cast<uint16_t>(pack_f16(v[i], 0.f));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (i < n) y[i * a.ld] = static_cast<uint16_t>(pack_bf16(v[i], 0.f));
+      }
     }
     __syncwarp();  // the next columns are loaded by the whole warp
   }
@@ -150,9 +140,8 @@ __device__ __forceinline__ void few_direct(const I8FewArgs& args, uint32_t tbase
 template <int NT, int STAGES>
 __global__ void __launch_bounds__(192, 1)
     gemm_i8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
-                       const I8FewArgs args) {
+                       const I8GemmArgs a) {
   using L = I8FewSmem<NT, STAGES>;
-  const I8GemmArgs& a = args.g;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -271,7 +260,7 @@ __global__ void __launch_bounds__(192, 1)
     const int ew = warp & 3;  // TMEM lanes 32 ew on: weight rows
     const uint32_t tbase = tmem_base + (static_cast<uint32_t>(ew * 32) << 16);
     if (splits == 1) {
-      few_direct<NT>(args, tbase, tile, ew, lane);
+      few_direct<NT>(a, tbase, tile, ew, lane);
     } else {
       const uint32_t dst = sbase + (ew * 32 + lane) * 4;
 #pragma unroll 1
@@ -368,9 +357,9 @@ __global__ void __launch_bounds__(192, 1)
             break;
           default: break;
         }
-        const long long o = m * args.ld + col;
+        const long long o = m * a.ld + col;
         if (add || a.epi == kEpiStoreF32) {
-          float* p = args.residual + o;
+          float* p = a.residual + o;
           if (two) {
             float2* p2 = reinterpret_cast<float2*>(p);
             *p2 = add ? fadd2(*p2, v) : v;
@@ -378,11 +367,9 @@ __global__ void __launch_bounds__(192, 1)
             *p = add ? *p + v.x : v.x;
           }
         } else if (two) {
-          *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(args.y) + o) = a.out_f16 ? pack_f16(v.x, v.y) : pack_bf16(v.x, v.y);
-        } else if (a.out_f16) {
-          static_cast<__half*>(args.y)[o] = __float2half_rn(v.x);
+          *reinterpret_cast<uint32_t*>(a.y + o) = a.out_f16 ? pack_f16(v.x, v.y) : pack_bf16(v.x, v.y);
         } else {
-          static_cast<__nv_bfloat16*>(args.y)[o] = __float2bfloat16_rn(v.x);
+          a.y[o] = static_cast<uint16_t>(a.out_f16 ? pack_f16(v.x, 0.f) : pack_bf16(v.x, 0.f));
         }
       }
     }

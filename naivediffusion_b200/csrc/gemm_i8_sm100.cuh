@@ -30,6 +30,9 @@ struct I8GemmArgs {
   long long gate_stride;
   const void* addend;
   long long ld_add;
+  uint16_t* y;        // 16-bit output, or
+  float* residual;    // the fp32 epilogues'
+  long long ld;       // its row stride
   uint32_t idesc;
   unsigned* status;
 };
@@ -190,8 +193,28 @@ __device__ __forceinline__ float2 i8_gelu_erf(float2 x) {
 // between two halves, fp32 ones take all of it. (Two 16-bit chunks as one store
 // of 128-byte rows from a single buffer: 4096 x 640 x 5120 GEGLU 35 -> 44 us;
 // three halves: no faster.)
-__device__ __forceinline__ void i8_emit(const CUtensorMap* tm, int kind, uint32_t buf, int& sb, int lane, int row0,
-                                        int col, const float2 (&v)[16]) {
+//
+// TMA clips a store's columns at 16 bytes, not at the tensor's width: where the
+// width ends inside 16 bytes, the output's last chunk is stored from the
+// registers instead, so that what lies beside it stays.
+__device__ __forceinline__ void i8_emit(const I8GemmArgs& a, const CUtensorMap* tm, int kind, int width, uint32_t buf, int& sb,
+                                        int lane, int row0, int col, const float2 (&v)[16]) {
+  if (col + 32 > width && (width & (kind == kEmitBf16 || kind == kEmitF16 ? 7 : 3)) != 0) {
+    if (row0 + lane < a.M) {
+      const long long o = (row0 + lane) * a.ld + col;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        if (col + i < width) {
+          const float f = (i & 1) ? v[i >> 1].y : v[i >> 1].x;
+          if (kind == kEmitF32) a.residual[o + i] = f;
+          else if (kind == kEmitAddF32) a.residual[o + i] += f;
+          else a.y[o + i] = static_cast<uint16_t>(kind == kEmitF16 ? pack_f16(f, 0.f) : pack_bf16(f, 0.f));
+        }
+      }
+    }
+    __syncwarp();
+    return;
+  }
   if (kind == kEmitBf16 || kind == kEmitF16) {
     buf += static_cast<uint32_t>(sb) * 2048u;
     sb ^= 1;
@@ -254,7 +277,7 @@ __device__ __forceinline__ void i8_chunk(const I8GemmArgs& a, const CUtensorMap*
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = fmul2(i8_silu(v[i]), g[i]);
     }
-    i8_emit(tmC, kind, buf, sb, lane, row0, ocol, v);
+    i8_emit(a, tmC, kind, a.half, buf, sb, lane, row0, ocol, v);
     return;
   }
   if (rows.mixed && a.bias) i8_own<false>(v, a.bias + (second ? a.bias_stride : 0) + ocol, a.N - ocol);
@@ -308,7 +331,7 @@ __device__ __forceinline__ void i8_chunk(const I8GemmArgs& a, const CUtensorMap*
     default:
       break;
   }
-  i8_emit(tmC, kind, buf, sb, lane, row0, ocol, v);
+  i8_emit(a, tmC, kind, a.N, buf, sb, lane, row0, ocol, v);
 }
 
 template <int BN, int STAGES>

@@ -49,9 +49,6 @@ struct I8GemvArgs {
   const int8_t* x;
   const int8_t* w;
   long long ldx, ldw;
-  void* y;          // 16-bit output, or
-  float* residual;  // the fp32 epilogues'
-  long long ld;
 };
 
 __device__ __forceinline__ float load_16bit(const void* p, long long i, int f16) {
@@ -59,7 +56,7 @@ __device__ __forceinline__ float load_16bit(const void* p, long long i, int f16)
 }
 
 template <int MR>
-__global__ void __launch_bounds__(kGemvI8Threads, MR == 2 ? 12 : 1) gemv_i8_kernel(const I8GemvArgs args) {
+__global__ void __launch_bounds__(kGemvI8Threads, MR == 1 ? 9 : MR == 2 ? 12 : 7) gemv_i8_kernel(const I8GemvArgs args) {
   constexpr int kGroups = MR == 2 ? 2 : 4;
   griddep_launch();
   griddep_wait();
@@ -147,11 +144,10 @@ __global__ void __launch_bounds__(kGemvI8Threads, MR == 2 ? 12 : 1) gemv_i8_kern
     case kEpiAddStore: v += load_16bit(a.addend, m * a.ld_add + col, a.out_f16); break;
     default: break;
   }
-  const long long at = m * args.ld + col;
-  if (a.epi == kEpiStoreF32) args.residual[at] = v;
-  else if (a.epi == kEpiResidualGate || a.epi == kEpiResidualAdd) args.residual[at] += v;
-  else if (a.out_f16) static_cast<__half*>(args.y)[at] = __float2half_rn(v);
-  else static_cast<__nv_bfloat16*>(args.y)[at] = __float2bfloat16_rn(v);
+  const long long at = m * a.ld + col;
+  if (a.epi == kEpiStoreF32) a.residual[at] = v;
+  else if (a.epi == kEpiResidualGate || a.epi == kEpiResidualAdd) a.residual[at] += v;
+  else a.y[at] = static_cast<uint16_t>(a.out_f16 ? pack_f16(v, 0.f) : pack_bf16(v, 0.f));
 }
 
 }  // namespace nd

@@ -183,21 +183,24 @@ def test_largest_sums_are_exact(cuda, m, n, k):
 
 
 @pytest.mark.parametrize("m", [1, 20, 50, 1200])
-def test_what_lies_beside_stays(cuda, m):
+@pytest.mark.parametrize("n", [200, 201, 7, 33, 389, 510])
+def test_what_lies_beside_stays(cuda, m, n):
     """Rows and columns past the output, and int8 columns past in_features, are neither written nor read."""
     from naivediffusion_b200 import ops
-    n, k = 200, 250
-    g = _gen(m)
+    k = 250
+    g = _gen(m + n)
     x, sx = _int8(g, m, k, pad=16)
     w, sw = _int8(g, n, k, pad=32)
-    for out, epi, dtype in ((None, "f32", F32), (BF16, "store", BF16)):
-        store = torch.full((m + 3, 232), 7.0, device="cuda", dtype=dtype)
-        args = dict(residual=store[:, :n]) if out is None else dict(out=store[:, :n])
-        ops.linear_w8a8(x, sx, w, sw, epilogue=EPI[epi], **args)
+    v, dv = linear64(x, sx, w, sw)
+    for epi, dtype in (("f32", F32), ("add", F32), ("store", BF16), ("gelu_tanh", F16)):
+        # negative zeros beside: adding nothing to them would show too
+        store = torch.full((m + 3, -(-n // 8) * 8 + 32), -0.0, device="cuda", dtype=dtype)
+        ops.linear_w8a8(x, sx, w, sw, epilogue=EPI[epi], **(dict(residual=store[:, :n]) if dtype == F32 else dict(out=store[:, :n])))
         ops.sync()
-        v, dv = linear64(x, sx, w, sw)
-        check(store[:m, :n], v, dv + (half_step(v.abs() + dv, dtype) if out else 0))
-        assert store[m:].eq(7).all() and store[:, n:].eq(7).all()
+        y, dy = act64(v, dv, epi) if epi == "gelu_tanh" else (v, dv)
+        check(store[:m, :n], y, dy + (half_step(y.abs() + dy, dtype) if dtype != F32 else U * y.abs()), epi)
+        beside = torch.cat([store[m:].flatten(), store[:m, n:].flatten()])
+        assert beside.eq(0).all() and torch.signbit(beside).all(), epi
 
 
 @pytest.mark.parametrize("m", [2, 17, 90, 1100])
