@@ -3,18 +3,22 @@
 //
 //   scale[r] = max |x[r]| / 127,   q[r, c] = rint(x[r, c] * 127 / max |x[r]|)
 //
-// The quotient is rounded as if computed exactly, half to even. The fast
-// product t = x * (127 / peak) is off by at most 2^-23 * 127; only where t lies
-// that near a half is its integer r checked against x * 127 - r * peak, which
-// two products and their fma remainders give exactly (near_half below). A
-// second pass over the thread's values with double division instead took 99 us
-// at 4352 x 12288: values of exactly half the peak make one in most rows.
+// The quotient is rounded as if computed exactly, half to even. 127 / peak is
+// held as a sum hi + lo of two fp32 values (2^-47 of it is missing), and
+// t = fma(x, hi, x * lo) is then the exact quotient rounded to fp32: a quotient
+// that is a half comes out as that half, and for 16-bit x any other differs
+// from a half by more than 1.9e-6 of itself, where t is off by 2^-24. Two fp32
+// values may have a quotient closer to a half than fp32 resolves; where t is a
+// half, x * 127 - r * peak decides, which two products and their fma remainders
+// give exactly (near_half). With 127 / peak in one fp32 value the near-half
+// check was needed for 16-bit x too (half the peak is common): 30 us at
+// 4352 x 12288 where this takes 26.
 //
 // Bound by HBM: the row is read once, stays in registers while its peak is
-// found, and one byte per value is written. 4352 x 12288 bf16 30 us (5.4 TB/s,
-// 82 % of the copy rate), 8192 x 8192 bf16 34 us (90 %); rows that are no
+// found, and one byte per value is written. 4352 x 12288 bf16 26 us (6.1 TB/s,
+// 93 % of the copy rate), 8192 x 8192 bf16 30 us, 4352 x 4096 fp32 14 us (98 %); rows that are no
 // multiple of 8 values are read a value at a time, four neighbours per thread
-// (1001 x 5121 fp32 7.6 us, 51 %; 4000 x 9001 bf16 47 us where one value per
+// (1001 x 5121 fp32 8.1 us, 48 %; 4000 x 9001 bf16 46 us where one value per
 // thread and store took 54).
 #include <algorithm>
 #include <climits>
@@ -27,9 +31,6 @@
 namespace nd {
 
 namespace {
-
-// The fast product x * (127 / peak) is off by at most 2^-23 * 127 = 1.5e-5.
-constexpr float kNearHalf = 0.49997f;
 
 // A thread's share of a row as it lies in memory: VEC values of one type. The
 // 16-bit types stay packed until they are quantized (half the registers, so
@@ -165,28 +166,44 @@ __device__ __forceinline__ float near_half(float x, float r, float peak) {
   return past > 0.f || (past == 0.f && odd) ? r + way : r;
 }
 
+// 127 / peak as hi + lo.
+struct Inverse {
+  float hi, lo;
+};
+__device__ __forceinline__ Inverse inverse_of(float peak) {
+  Inverse v;
+  v.hi = __fdiv_rn(127.0f, peak);
+  v.lo = __fdiv_rn(fmaf(-v.hi, peak, 127.0f), peak);  // the remainder is exact
+  return v;
+}
+
 // VEC values (already multiplied by `shift`'s power of two) to int8, of which n exist.
-template <int VEC>
-__device__ __forceinline__ void quantize_store(int8_t* q, const float (&f)[VEC], float inverse, float peak, int n) {
+template <int TYPE, int VEC>
+__device__ __forceinline__ void quantize_store(int8_t* q, const float (&f)[VEC], Inverse inv, float peak, int n) {
   float m[VEC];  // rint(t) + 1.5 * 2^23
   float most = 0.f;
   if constexpr (VEC > 1) {
-    const float2 inv2 = make_float2(inverse, inverse), magic2 = make_float2(kRintMagic, kRintMagic);
+    const float2 hi2 = make_float2(inv.hi, inv.hi), lo2 = make_float2(inv.lo, inv.lo);
+    const float2 magic2 = make_float2(kRintMagic, kRintMagic);
 #pragma unroll
     for (int j = 0; j < VEC; j += 2) {
       const float2 x2 = make_float2(f[j], f[j + 1]);
-      const float2 m2 = ffma2(x2, inv2, magic2);
-      const float2 r2 = fadd2(magic2, make_float2(-m2.x, -m2.y));
-      const float2 off = ffma2(x2, inv2, r2);
+      const float2 t2 = ffma2(x2, hi2, fmul2(x2, lo2));
+      const float2 m2 = fadd2(t2, magic2);
+      if constexpr (TYPE == ND_F32) {
+        const float2 r2 = fadd2(magic2, make_float2(-m2.x, -m2.y));
+        const float2 off = fadd2(t2, r2);
+        most = fmax3(most, fabsf(off.x), fabsf(off.y));
+      }
       m[j] = m2.x;
       m[j + 1] = m2.y;
-      most = fmax3(most, fabsf(off.x), fabsf(off.y));
     }
   } else {
-    m[0] = fmaf(f[0], inverse, kRintMagic);
-    most = fabsf(fmaf(f[0], inverse, kRintMagic - m[0]));
+    const float t = fmaf(f[0], inv.hi, f[0] * inv.lo);
+    m[0] = t + kRintMagic;
+    most = fabsf(t - (m[0] - kRintMagic));
   }
-  if (most > kNearHalf) {
+  if (TYPE == ND_F32 && most == 0.5f) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) m[j] = near_half(f[j], m[j] - kRintMagic, peak) + kRintMagic;
   }
@@ -256,14 +273,14 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T, (TYPE == ND_F32 && VEC == 8
   if (s.inverse == 0.f) {  // zeros, or infinities and NaN: every q is 0
     const float zero[VEC] = {};
 #pragma unroll 1
-    for (int c = t * VEC; c < width; c += T * VEC) quantize_store<VEC>(out + c, zero, 0.f, 1.f, width - c);
+    for (int c = t * VEC; c < width; c += T * VEC) quantize_store<TYPE, VEC>(out + c, zero, Inverse{0.f, 0.f}, 1.f, width - c);
     return;
   }
   // Where 127 / peak or 127 x would leave fp32's range, the row is worked on
   // times a power of two (which changes no quotient).
   const float shift = s.peak < 1e-30f ? 0x1p96f : s.peak > 1e30f ? 0x1p-64f : 1.f;
   const float row_peak = s.peak * shift;
-  const float inverse = shift == 1.f ? s.inverse : __fdiv_rn(127.0f, row_peak);
+  const Inverse inverse = inverse_of(row_peak);
   auto finish = [&](int c, const Raw<TYPE, VEC>& raw) {
     float w[VEC];
     raw.values(w);
@@ -271,7 +288,7 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T, (TYPE == ND_F32 && VEC == 8
 #pragma unroll
       for (int j = 0; j < VEC; ++j) w[j] *= shift;
     }
-    quantize_store<VEC>(out + c, w, inverse, row_peak, width - c);
+    quantize_store<TYPE, VEC>(out + c, w, inverse, row_peak, width - c);
   };
 #pragma unroll
   for (int i = 0; i < V; ++i) {
