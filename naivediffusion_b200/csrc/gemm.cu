@@ -550,22 +550,19 @@ int dequantize(const int8_t* q, const void* scales, int scale_dtype, int64_t qua
   const int64_t group = quant_group > 0 ? quant_group : cols;
   if (cols % group) return fail(ND_ERR_INVALID, "dequantize: quant_group must divide cols");
   const bool aligned = reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
-  const bool by16 = aligned && cols % 16 == 0 && group % 16 == 0;
   const int64_t runs = (rows * cols + 16 * 256 - 1) / (16 * 256);
-  if (aligned && !by16 && group == cols && cols >= 16 && runs <= INT_MAX) {
-    dequant_rows_kernel<<<static_cast<unsigned>(runs), 256, 0, stream>>>(q, scales, scale_dtype == ND_F16, rows * cols,
-                                                                         static_cast<int>(cols), static_cast<uint16_t*>(out),
-                                                                         out_dtype == ND_F16);
-    ND_CUDA(cudaGetLastError());
-    return ND_OK;
+  const int f16 = scale_dtype == ND_F16, g = static_cast<int>(group), w = static_cast<int>(cols);
+  uint16_t* o = static_cast<uint16_t*>(out);
+  if (aligned && group >= 16 && runs <= INT_MAX) {
+    dequant_runs_kernel<<<static_cast<unsigned>(runs), 256, 0, stream>>>(q, scales, f16, rows * cols, g, o, out_dtype == ND_F16);
+  } else {
+    const int64_t per_row = (cols + 127) / 128;  // blocks to cover a row at once
+    const int64_t most = sm_count() * 16LL;
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(rows, most)),
+                    static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(per_row, most / std::min<int64_t>(rows, most)))));
+    dequant_w8_kernel<<<grid, 128, 0, stream>>>(q, scales, f16, g, static_cast<int>(cols / group), rows, w, o,
+                                                out_dtype == ND_F16);
   }
-  const int64_t per_row = (cols + (by16 ? 16 * 128 : 128) - 1) / (by16 ? 16 * 128 : 128);  // blocks to cover a row at once
-  const int64_t most = sm_count() * 16LL;
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(rows, most)),
-                  static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(per_row, most / std::min<int64_t>(rows, most)))));
-  const int f16 = scale_dtype == ND_F16, g = static_cast<int>(group), sc = static_cast<int>(cols / group), w = static_cast<int>(cols);
-  if (by16) dequant_w8_kernel<16><<<grid, 128, 0, stream>>>(q, scales, f16, g, sc, rows, w, out, out_dtype == ND_F16);
-  else dequant_w8_kernel<1><<<grid, 128, 0, stream>>>(q, scales, f16, g, sc, rows, w, out, out_dtype == ND_F16);
   ND_CUDA(cudaGetLastError());
   return ND_OK;
 }

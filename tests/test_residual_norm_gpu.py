@@ -262,6 +262,23 @@ def test_values_of_int8_rows(cuda, rows, cols, dtype):
     check(got, v, s * 0.5 + 2 * U * v.abs() + half_step(v.abs() + s, dtype))
 
 
+@pytest.mark.parametrize("rows,cols,group", [(300, 512, 32), (301, 264, 24), (77, 340, 20), (5, 51, 17), (129, 96, 16),
+                                             (64, 640, 8), (3, 15, 5), (2000, 2560, 64), (1, 33, 33)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_values_of_groups(cuda, rows, cols, group, dtype):
+    """Groups that runs of 16 values straddle, and matrices off a 16-byte address, bit for bit."""
+    from naivediffusion_b200 import ops
+    g = _gen(rows + cols)
+    q = torch.randint(-127, 128, (rows * cols + 3,), generator=g, device=g.device, dtype=I8).cuda()
+    scale = _randn(g, rows, cols // group).cuda().abs()
+    for start, sdt in ((0, F32), (0, F16), (3, F32)):
+        part, s = q[start:start + rows * cols].view(rows, cols), scale.to(sdt)
+        got = ops.dequantize(part, s, group, dtype)
+        ops.sync()
+        want = (part.float().view(rows, -1, group) * s.float()[:, :, None]).to(dtype)
+        assert torch.equal(got, want.view(rows, cols))
+
+
 def test_streams_and_graphs(cuda):
     """On a side stream, and captured: a replay reads the inputs' values of that moment."""
     from naivediffusion_b200 import ops
