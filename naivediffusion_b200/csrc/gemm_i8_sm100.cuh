@@ -174,9 +174,11 @@ __device__ __forceinline__ float2 i8_gelu_tanh(float2 x) {
 // Exact GELU, x (1 + erf(x / sqrt 2)) / 2 = max(x, 0) - |x| erfc(|x| / sqrt 2) / 2,
 // with erfc(z) = (a1 t + .. + a5 t^5) exp(-z^2), t = 1 / (1 + p z): Abramowitz
 // and Stegun 7.1.26, off by at most 1.5e-7, the form the reference's
-// CpuMath.Gelu has. Half the instructions of erff.
+// CpuMath.Gelu has. Half the instructions of erff. +inf counts as the largest
+// finite |x|, whose erfc is 0 too: the last product would be inf * 0.
 __device__ __forceinline__ float2 i8_gelu_erf(float2 x) {
-  const float2 ax = make_float2(fabsf(x.x), fabsf(x.y));
+  constexpr float kMost = 3.402823466e38f;
+  const float2 ax = make_float2(fabsf(fminf(x.x, kMost)), fabsf(fminf(x.y, kMost)));
   const float2 d = ffma2(ax, splat(0.3275911f * 0.70710678118654752f), splat(1.f));
   const float2 t = make_float2(fast_rcp(d.x), fast_rcp(d.y));
   float2 p = ffma2(t, splat(1.061405429f), splat(-1.453152027f));

@@ -320,3 +320,29 @@ def test_a_block_of_them(cuda):
     # factor's relative error on with a slope below 2 (variance 4) from each of its factors, and the hidden rows' peak is
     # below 40 of their deviations: 8.3e-3. Together under 1.5e-2 of the variance: cosine above 1 - 0.75e-2.
     assert cos > 0.9925, cos
+
+
+@pytest.mark.parametrize("m", [1, 3, 20, 100, 300, 1100])
+@pytest.mark.parametrize("act", ["gelu_tanh", "gelu_erf", "silu", "swiglu", "geglu"])
+def test_activations_of_infinities(cuda, m, act):
+    """An infinite bias, and a scaled sum that overflows: +inf stays +inf and what the definition makes NaN is NaN."""
+    from naivediffusion_b200 import ops
+    n, k = 256, 320
+    _, x, sx, w, sw, b = _case(m, n, k, m + 23, gated=act in ("swiglu", "geglu"))
+    b[5::16], b[6::32] = math.inf, -math.inf
+    sx[m // 2] = 3e38
+    sw[9::16] = 1e3
+    y = ops.linear_w8a8(x, sx, w, sw, b, epilogue=EPI[act])
+    ops.sync()
+    v = (linear64(x, sx, w, sw, b)[0]).float().double()  # overflows where fp32 does
+    f = n if act in ("swiglu", "geglu") else v.shape[1]
+    zero = torch.zeros((), device="cuda", dtype=torch.float64)
+    if act == "swiglu":
+        want = act64(v[:, :f], zero, "silu")[0] * v[:, f:]
+    elif act == "geglu":
+        want = v[:, :f] * act64(v[:, f:], zero, "gelu_erf")[0]
+    else:
+        want = act64(v, zero, act)[0]
+    far = torch.isinf(want)
+    assert far.any() and torch.equal(torch.isnan(y), torch.isnan(want))
+    assert torch.equal(y[far].double(), want[far])
