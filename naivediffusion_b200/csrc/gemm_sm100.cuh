@@ -171,8 +171,9 @@ __device__ __forceinline__ void load_vec32(const float* src, int col, int N, flo
 // Stage one warp's [32 rows x 32 columns] chunk (lane = row) in shared memory
 // in the tensor map's swizzled layout and hand it to TMA: a store (bf16, fp16,
 // fp32, or a bf16 hi|lo pair whose lo chunk goes to column col + lo_off) or
-// an fp32 reduce-add into global memory. Rows / columns past the tensor's
-// edge are clipped by TMA. Two staging buffers per warp alternate; a buffer is
+// an fp32 reduce-add into global memory. Rows past the tensor's edge are
+// clipped by TMA, columns at the next multiple of 16 bytes (store_tail takes
+// the chunk where that is not the width). Two staging buffers per warp alternate; a buffer is
 // rewritten only after the store issued from it two chunks ago has finished
 // reading it.
 __device__ __forceinline__ void emit_chunk(const CUtensorMap* tm, int kind, uint32_t buf0, int& sb,
@@ -232,6 +233,29 @@ __device__ __forceinline__ void emit_chunk(const CUtensorMap* tm, int kind, uint
     else tma_store_2d(tm, buf, col, row0);
     bulk_commit();
   }
+}
+
+// TMA clips a store's columns at 16 bytes, not at the tensor's width. Where the
+// width ends inside 16 bytes this stores the output's last chunk from the
+// registers (lane = row), so that what lies beside it stays, and returns true.
+// Plain epilogues only: the others' widths are multiples of 32 columns.
+__device__ __forceinline__ bool store_tail(const GemmArgs& a, int kind, int lane, int row0, int col, const float (&v)[32]) {
+  const bool f32 = kind == kEmitF32 || kind == kEmitAddF32;
+  if (col + 32 <= a.N || kind == kEmitSplit || (a.N & (f32 ? 3 : 7)) == 0) return false;
+  const long long row = row0 + lane;
+  if (row < a.M) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      if (col + i >= a.N) continue;
+      if (kind == kEmitF32) a.resid[row * a.ldr + col + i] = v[i];
+      else if (kind == kEmitAddF32) a.resid[row * a.ldr + col + i] += v[i];
+      else
+        static_cast<uint16_t*>(a.out)[row * a.ldo + col + i] =
+            static_cast<uint16_t>(kind == kEmitF16 ? pack_f16(v[i], 0.f) : pack_bf16(v[i], 0.f));
+    }
+  }
+  __syncwarp();
+  return true;
 }
 
 // One 32-column chunk of a plain epilogue (everything but kEpiQkNormRope).
@@ -303,6 +327,7 @@ __device__ __forceinline__ void epilogue_chunk(const GemmArgs& a, const CUtensor
     default:
       break;
   }
+  if (store_tail(a, kind, lane, row0, col, v)) return;
   emit_chunk(tmC, kind, buf0, sb, lane, row0, a.M, col, v, a.N);
 }
 
