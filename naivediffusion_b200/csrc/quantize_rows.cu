@@ -151,62 +151,11 @@ __device__ __forceinline__ uint32_t peak_bits(uint32_t m) {
   else return __float_as_uint(halves<TYPE>(max(m & 0xffffu, m >> 16)).x);
 }
 
-// The exact rounding of x * 127 / peak, given r, its integer by the fast
-// product, where the quotient lies near r +- 1/2. 127 x = hi + lo and
-// r peak = hi2 + lo2 exactly (fma remainders); hi - hi2, 2 |d| - peak and
-// lo - lo2 are differences of near neighbours or of few bits and exact, so the
-// sign of their sum says on which side of the half the quotient lies.
-__device__ __forceinline__ float near_half(float x, float r, float peak) {
-  const float hi = x * 127.0f, lo = fmaf(x, 127.0f, -hi);
-  const float hi2 = r * peak, lo2 = fmaf(r, peak, -hi2);
-  const float d = hi - hi2;
-  const float way = d < 0.f ? -1.f : 1.f;
-  const float past = (2.f * fabsf(d) - peak) + 2.f * way * (lo - lo2);
-  const bool odd = (__float2int_rn(r) & 1) != 0;
-  return past > 0.f || (past == 0.f && odd) ? r + way : r;
-}
-
-// 127 / peak as hi + lo.
-struct Inverse {
-  float hi, lo;
-};
-__device__ __forceinline__ Inverse inverse_of(float peak) {
-  Inverse v;
-  v.hi = __fdiv_rn(127.0f, peak);
-  v.lo = __fdiv_rn(fmaf(-v.hi, peak, 127.0f), peak);  // the remainder is exact
-  return v;
-}
-
-// VEC values (already multiplied by `shift`'s power of two) to int8, of which n exist.
+// VEC values (already multiplied by range_shift) to int8, of which n exist.
 template <int TYPE, int VEC>
 __device__ __forceinline__ void quantize_store(int8_t* q, const float (&f)[VEC], Inverse inv, float peak, int n) {
-  float m[VEC];  // rint(t) + 1.5 * 2^23
-  float most = 0.f;
-  if constexpr (VEC > 1) {
-    const float2 hi2 = make_float2(inv.hi, inv.hi), lo2 = make_float2(inv.lo, inv.lo);
-    const float2 magic2 = make_float2(kRintMagic, kRintMagic);
-#pragma unroll
-    for (int j = 0; j < VEC; j += 2) {
-      const float2 x2 = make_float2(f[j], f[j + 1]);
-      const float2 t2 = ffma2(x2, hi2, fmul2(x2, lo2));
-      const float2 m2 = fadd2(t2, magic2);
-      if constexpr (TYPE == ND_F32) {
-        const float2 r2 = fadd2(magic2, make_float2(-m2.x, -m2.y));
-        const float2 off = fadd2(t2, r2);
-        most = fmax3(most, fabsf(off.x), fabsf(off.y));
-      }
-      m[j] = m2.x;
-      m[j + 1] = m2.y;
-    }
-  } else {
-    const float t = fmaf(f[0], inv.hi, f[0] * inv.lo);
-    m[0] = t + kRintMagic;
-    most = fabsf(t - (m[0] - kRintMagic));
-  }
-  if (TYPE == ND_F32 && most == 0.5f) {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) m[j] = near_half(f[j], m[j] - kRintMagic, peak) + kRintMagic;
-  }
+  float m[VEC];
+  quantize_values<TYPE == ND_F32>(f, inv, peak, m);
   if constexpr (VEC == 8) {
     *reinterpret_cast<uint2*>(q) =
         make_uint2(pack_low_bytes(__float_as_uint(m[0]), __float_as_uint(m[1]), __float_as_uint(m[2]), __float_as_uint(m[3])),
@@ -270,15 +219,13 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T, (TYPE == ND_F32 && VEC == 8
   const RowScale s = row_scale(block_max<T>(peak_bits<TYPE>(peak), red));
   if (t == 0) scale[r] = s.scale;
   int8_t* out = q + r * ldq;
-  if (s.inverse == 0.f) {  // zeros, or infinities and NaN: every q is 0
+  if (s.zero) {
     const float zero[VEC] = {};
 #pragma unroll 1
     for (int c = t * VEC; c < width; c += T * VEC) quantize_store<TYPE, VEC>(out + c, zero, Inverse{0.f, 0.f}, 1.f, width - c);
     return;
   }
-  // Where 127 / peak or 127 x would leave fp32's range, the row is worked on
-  // times a power of two (which changes no quotient).
-  const float shift = s.peak < 1e-30f ? 0x1p96f : s.peak > 1e30f ? 0x1p-64f : 1.f;
+  const float shift = range_shift(s.peak);
   const float row_peak = s.peak * shift;
   const Inverse inverse = inverse_of(row_peak);
   auto finish = [&](int c, const Raw<TYPE, VEC>& raw) {

@@ -15,7 +15,8 @@
 // written once; the row stays in registers between its (up to five) row-wide
 // reductions. Variances are centred second moments over the registers, in
 // fp32. 4352 x 4096 (bf16 branch and y) 39 us, 5.5 TB/s, 83 % of the copy rate;
-// 8192 x 2048 to int8 34 us, 82 %; 4000 x 3001 41 us, 54 %.
+// 8192 x 2048 to int8 36 us, 79 % (34 with one fp32 factor 127 / peak, whose
+// int8 rows were one off quantize_rows' near halves); 4000 x 3001 41 us, 54 %.
 #include <algorithm>
 #include <climits>
 
@@ -310,19 +311,28 @@ __device__ __forceinline__ void finish_row(const ResidualNorm& a, long long r, i
                    max(abs_bits(v[2 * i + 1].x), abs_bits(v[2 * i + 1].y)));
       else peak = max(peak, abs_bits(i & 1 ? v[i / 2].y : v[i / 2].x));
     }
-  // y is an fp32 result already, so the quotient's last bit decides nothing
-  // that fp32 had not rounded before: multiply by 127 / peak.
   const RowScale s = row_scale(row_max<T>(peak, reinterpret_cast<uint32_t*>(red[4])));
   if (t == 0) a.y_scale[r] = s.scale;
-  // Where 127 / peak leaves fp32's range, both are first multiplied up.
-  const bool tiny = s.inverse != 0.f && s.peak < 1e-30f;
-  const float inverse = tiny ? __fdiv_rn(127.0f, s.peak * 0x1p96f) : s.inverse;
-  if (tiny) {
+  if (s.zero) {
 #pragma unroll
-    for (int h = 0; h < S::H; ++h) v[h] = fmul2(v[h], splat(0x1p96f));
+    for (int h = 0; h < S::H; ++h) v[h] = splat(kRintMagic);
+  } else {
+    const float shift = range_shift(s.peak);
+    if (shift != 1.f) {
+#pragma unroll
+      for (int h = 0; h < S::H; ++h) v[h] = fmul2(v[h], splat(shift));
+    }
+    const float row_peak = s.peak * shift;
+    const Inverse inverse = inverse_of(row_peak);
+#pragma unroll
+    for (int h = 0; h < S::H; h += 2) {
+      const float f[4] = {v[h].x, v[h].y, v[h + 1].x, v[h + 1].y};
+      float m[4];
+      quantize_values<true>(f, inverse, row_peak, m);
+      v[h] = make_float2(m[0], m[1]);
+      v[h + 1] = make_float2(m[2], m[3]);
+    }
   }
-#pragma unroll
-  for (int h = 0; h < S::H; ++h) v[h] = s.inverse != 0.f ? ffma2(v[h], splat(inverse), splat(kRintMagic)) : splat(kRintMagic);
   S::store(static_cast<int8_t*>(a.y) + r * a.ldy + first, rem, v);
 }
 

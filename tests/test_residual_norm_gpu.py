@@ -339,3 +339,35 @@ def test_many_rows_in_place_on_two_streams_and_captured(cuda, rows, width):
         graph.replay()
         ops.sync()
         assert new is x and torch.equal(x, want[0][step][0]) and torch.equal(y, want[0][step][1])
+
+
+@pytest.mark.parametrize("rows,width", [(1, 1), (9, 4), (40, 130), (33, 512), (30, 1024), (20, 1155), (64, 2048), (7, 4100), (5, 8192),
+                                        (2, 12289), (2, 16384), (5000, 2048), (3000, 2047), (17000, 512), (1100, 8192)])
+@pytest.mark.parametrize("pre", [NONE, RMS, LAYER])
+def test_int8_rows_are_those_of_the_quantizer(cuda, rows, width, pre):
+    """An int8 y is what quantize_rows makes of the fp32 y, bit for bit; every quotient a half or near one without a norm."""
+    from naivediffusion_b200 import ops
+    g = _gen(rows + width + pre)
+    if pre == NONE:  # peak 381 2^j, so y * 127 / peak = y 2^-j / 3: thirds of odd halves, and their neighbours
+        x = (torch.randint(-762, 763, (rows, width), generator=g, device="cuda").float() / 2)
+        x[:, 0] = 381
+        near = torch.nextafter(x, torch.where(x > 0, math.inf, -math.inf).to(x))
+        x = torch.where(torch.rand(rows, width, generator=g, device="cuda") < 0.25, near.clamp(-381, 381), x)
+        x = x * 2.0 ** torch.randint(-120, 110, (rows, 1), generator=g, device="cuda")
+    else:
+        x = _randn(g, rows, width) * 2 + 0.5
+    x[rows // 2] = 0
+    _, y = ops.residual_norm(x, pre_norm=pre, out_dtype=F32)
+    _, q, scale = ops.residual_norm(x, pre_norm=pre, out_dtype=I8)
+    want, ws = ops.quantize_rows(y)
+    ops.sync()
+    assert torch.equal(scale, ws)
+    assert torch.equal(q, want), (q != want).sum()
+
+
+def test_an_exact_half_goes_to_even(cuda):
+    from naivediffusion_b200 import ops
+    x = torch.tensor([[381.0, 1.5, -1.5, 4.5, -4.5, 7.5]], device="cuda")
+    _, q, scale = ops.residual_norm(x, pre_norm=NONE, out_dtype=I8)
+    ops.sync()
+    assert q[0].tolist() == [127, 0, 0, 2, -2, 2] and scale[0] == 3
