@@ -136,15 +136,17 @@ __device__ __forceinline__ void i8_scaled(const uint32_t (&r)[32], float sx, uin
   }
 }
 
-// v (op) this lane's own 32 values in global memory, of which n exist: a
-// straddling warp's bias (add) and gate (multiply).
-template <bool MUL>
-__device__ __forceinline__ void i8_own(float2 (&v)[16], const float* own, int n) {
+// This lane's own 32 values in global memory, of which n exist, for a warp that
+// straddles the split: its bias, v * sx + bias (v: sums times w_scale, not yet
+// times sx, so that a row is rounded as often as in any other warp), or its gate,
+// v * gate.
+template <bool GATE>
+__device__ __forceinline__ void i8_own(float2 (&v)[16], float sx, const float* own, int n) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) {
     const float f = i < n ? __ldg(own + i) : 0.f;
     float& t = (i & 1) ? v[i >> 1].y : v[i >> 1].x;
-    t = MUL ? t * f : t + f;
+    t = GATE ? t * f : fmaf(t, sx, f);
   }
 }
 
@@ -262,15 +264,17 @@ __device__ __forceinline__ void i8_chunk(const I8GemmArgs& a, const CUtensorMap*
   const int row = row0 + lane;
   const bool second = row >= a.group_split;  // read by straddling warps only
   int kind = a.out_f16 ? kEmitF16 : kEmitBf16;
+  const bool own_bias = rows.mixed && a.bias;
+  const float sx1 = own_bias ? 1.f : sx;  // the staged bias is 0 then: sum * w_scale comes out as it is
   float2 v[16];
-  i8_scaled(r, sx, vecs + 4 * lc, v);
+  i8_scaled(r, sx1, vecs + 4 * lc, v);
   if (a.half > 0) {
     float2 g[16];
-    i8_scaled(r2, sx, vecs + 4 * (64 + lc), g);
-    if (rows.mixed && a.bias) {
+    i8_scaled(r2, sx1, vecs + 4 * (64 + lc), g);
+    if (own_bias) {
       const float* own = a.bias + (second ? a.bias_stride : 0) + ocol;
-      i8_own<false>(v, own, a.half - ocol);
-      i8_own<false>(g, own + a.half, a.half - ocol);
+      i8_own<false>(v, sx, own, a.half - ocol);
+      i8_own<false>(g, sx, own + a.half, a.half - ocol);
     }
     if (a.epi == kEpiGeGlu) {
 #pragma unroll
@@ -282,7 +286,7 @@ __device__ __forceinline__ void i8_chunk(const I8GemmArgs& a, const CUtensorMap*
     i8_emit(a, tmC, kind, a.half, buf, sb, lane, row0, ocol, v);
     return;
   }
-  if (rows.mixed && a.bias) i8_own<false>(v, a.bias + (second ? a.bias_stride : 0) + ocol, a.N - ocol);
+  if (own_bias) i8_own<false>(v, sx, a.bias + (second ? a.bias_stride : 0) + ocol, a.N - ocol);
   switch (a.epi) {
     case kEpiGeluTanh:
 #pragma unroll
@@ -298,7 +302,7 @@ __device__ __forceinline__ void i8_chunk(const I8GemmArgs& a, const CUtensorMap*
       break;
     case kEpiResidualGate:
       if (rows.mixed) {
-        i8_own<true>(v, a.gate + (second ? a.gate_stride : 0) + ocol, a.N - ocol);
+        i8_own<true>(v, 1.f, a.gate + (second ? a.gate_stride : 0) + ocol, a.N - ocol);
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {

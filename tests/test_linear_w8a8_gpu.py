@@ -346,3 +346,27 @@ def test_activations_of_infinities(cuda, m, act):
     far = torch.isinf(want)
     assert far.any() and torch.equal(torch.isnan(y), torch.isnan(want))
     assert torch.equal(y[far].double(), want[far])
+
+
+@pytest.mark.parametrize("m,splits", [(3, (1, 2)), (30, (7, 16)), (200, (33, 77)), (1500, (130, 1003))])
+@pytest.mark.parametrize("act", ["f32", "store", "gate", "gelu_erf", "swiglu"])
+def test_a_split_changes_no_row(cuda, m, splits, act):
+    """With shared weights a row's bits do not depend on where the two groups meet: they are those of its own group's
+    vectors alone."""
+    from naivediffusion_b200 import ops
+    n, k = 256, 384
+    g, x, sx, w, sw, _ = _case(m, n, k, m + 41, gated=act == "swiglu")
+    b = torch.randn(2, w.shape[0], generator=g, device="cuda")
+    gate = torch.randn(2, n, generator=g, device="cuda") if act == "gate" else None
+    r0 = torch.randn(m, n, generator=g, device="cuda")
+
+    def run(bias, gates, **kw):
+        if act == "gate":
+            kw.update(gate=gates, residual=r0.clone())
+        return ops.linear_w8a8(x, sx, w, sw, bias, epilogue=EPI[act], **kw)
+
+    alone = [run(b[i], None if gate is None else gate[i]) for i in range(2)]
+    for split in splits:
+        y = run(b, gate, group_split=split, shared_weights=True)
+        ops.sync()
+        assert torch.equal(y[:split], alone[0][:split]) and torch.equal(y[split:], alone[1][split:]), split
