@@ -61,7 +61,8 @@ __global__ void __launch_bounds__(kGemvI8Threads, MR == 1 ? 9 : MR == 2 ? 12 : 7
   griddep_launch();
   griddep_wait();
   const I8GemmArgs& a = args.g;
-  const int warp = (blockIdx.x * kGemvI8Threads + threadIdx.x) >> 5;
+  // Blocks times warps: the threads' own numbers pass 32 bits at 2^27 gated outputs.
+  const int warp = static_cast<int>(blockIdx.x) * (kGemvI8Threads / 32) + static_cast<int>(threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   const bool gated = a.half > 0;
   const int n0 = gated ? warp : 2 * warp;

@@ -370,3 +370,21 @@ def test_a_split_changes_no_row(cuda, m, splits, act):
         y = run(b, gate, group_split=split, shared_weights=True)
         ops.sync()
         assert torch.equal(y[:split], alone[0][:split]) and torch.equal(y[split:], alone[1][split:]), split
+
+
+def test_more_gated_outputs_than_warps_count_in_32_bits(cuda):
+    """One row, 2^27 + 128 outputs: a warp each, whose threads' numbers pass 2^32."""
+    from naivediffusion_b200 import ops
+    n, k = (1 << 27) + 128, 16
+    x, sx = torch.ones(1, k, device="cuda", dtype=I8), torch.ones(1, device="cuda")
+    w = torch.ones(2 * n, k, device="cuda", dtype=I8)
+    sw = torch.full((2 * n,), 1 / 16, device="cuda")
+    sw[n - 100:n], sw[n:n + 50] = 1 / 8, 1 / 4  # first factors 2 at the end, second factors 4 at the start
+    out = torch.full((1, n), math.nan, device="cuda", dtype=BF16)
+    ops.linear_w8a8(x, sx, w, sw, epilogue=EPI["swiglu"], out=out)
+    ops.sync()
+    one, two = (1 / (1 + math.exp(-1))), 2 / (1 + math.exp(-2))
+    want = torch.full((n,), one, device="cuda", dtype=F32)
+    want[:50], want[n - 100:] = 4 * one, two
+    # two fp32 roundings of the factors, ex2 and rcp a few ulp each, and the store's half step
+    assert (out[0].float() - want).abs().le(want * (2.0 ** -8 + 16 * U)).all()
