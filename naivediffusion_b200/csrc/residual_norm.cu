@@ -472,7 +472,8 @@ __global__ void __launch_bounds__(T, CTAS) residual_norm_ring_kernel(const Resid
   bool ok = true;
   for (int r = blockIdx.x; r < a.rows; r += step, ++it) {
     if (t < 32) ok = mbar_wait(smem_u32(&full_bars[s]), parity, &abort_flag, status, kStatusTimeoutProducer);
-    if (!__syncthreads_and(ok)) break;
+    ok = __syncthreads_and(ok);  // the block's: thread 0 sees another lane's timeout too
+    if (!ok) break;
     // Everyone is done with the row before this one: its slot is filled again.
     if (t == 0 && it > 0 && next < a.rows) fetch(s > 0 ? s - 1 : slots - 1);
     if (r >= vec_end) {
