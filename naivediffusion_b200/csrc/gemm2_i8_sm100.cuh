@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(kI8PairThreads, 1)
       const int col0 = nt * per_tile + side * (per_tile / 2);
       const float sx = row0 + lane < args.M ? __ldg(args.x_scale + row0 + lane) : 0.f;
       if (row0 < args.M) i8_stage_vectors(args, vecs, wgroup, rows, col0, lane);
-      if (!mbar_wait(accf_bar(acc), (local >> 1) & 1, abort_flag, args.status, kStatusTimeoutEpilogue)) break;
+      if (!mbar_wait_warp(accf_bar(acc), (local >> 1) & 1, abort_flag, args.status, kStatusTimeoutEpilogue)) break;
       __syncwarp();
       tc_fence_after();
       const uint32_t tbase = tmem_base + (static_cast<uint32_t>(ew * 32) << 16) + acc * BN;

@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(192, 1)
       volatile int never = 0;
       mbar_wait(drain_bar, 0, &never, a.status, kStatusTimeoutDrain);
     }
-  } else if (mbar_wait(accf_bar, 0, abort_flag, a.status, kStatusTimeoutEpilogue)) {
+  } else if (mbar_wait_warp(accf_bar, 0, abort_flag, a.status, kStatusTimeoutEpilogue)) {
     __syncwarp();
     tc_fence_after();
     const int ew = warp & 3;  // TMEM lanes 32 ew on: weight rows

@@ -53,6 +53,14 @@ __device__ __forceinline__ void umma_ss_i8(uint32_t d_tmem, uint64_t a_desc, uin
       : "memory");
 }
 
+// A whole warp's wait: true only where every lane's is, so that after a timeout
+// no part of the warp goes on alone into tcgen05 instructions that all of it
+// has to run.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort, unsigned* status,
+                                               unsigned where) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, status, where));
+}
+
 // ------------------------------------------------------------ epilogue
 // A warp's columns of the per-column vectors, staged in its own shared memory
 // while the tile's MMAs run. With that, the paired fp32 arithmetic and the ex2 /
@@ -507,7 +515,7 @@ __global__ void __launch_bounds__(192, 1)
     const int per_tile = args.half > 0 ? BN / 2 : BN;
     const int col0 = nt * per_tile;
     if (row0 < args.M && splits == 1) i8_stage_vectors(args, vecs, wgroup, rows, col0, lane);
-    if (row0 < args.M && mbar_wait(accf_bar, 0, abort_flag, args.status, kStatusTimeoutEpilogue)) {
+    if (row0 < args.M && mbar_wait_warp(accf_bar, 0, abort_flag, args.status, kStatusTimeoutEpilogue)) {
       __syncwarp();
       tc_fence_after();
       const uint32_t tbase = tmem_base + (static_cast<uint32_t>(ew * 32) << 16);
