@@ -310,7 +310,7 @@ _FP32, _INT8, _HALVES = (_F32,), (_I8,), (torch.bfloat16, torch.float16)
 def residual_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *, x_out: torch.Tensor | None = None,
                   post_norm: int = _lib.ND_NORM_NONE, post_weight: torch.Tensor | None = None,
                   gate: torch.Tensor | None = None, residual_scale: float = 1.0,
-                  pre_norm: int = _lib.ND_NORM_LAYER, pre_weight: torch.Tensor | None = None,
+                  pre_norm: int | None = None, pre_weight: torch.Tensor | None = None,
                   scale: torch.Tensor | None = None, shift: torch.Tensor | None = None, rows_per_vec: int = 0,
                   plus_one: bool = False, eps: float = 1e-6, out_dtype=torch.bfloat16,
                   out: torch.Tensor | None = None, out_scale: torch.Tensor | None = None):
@@ -319,7 +319,8 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *, x_out:
     x: fp32 [rows, width], updated in place unless x_out is given (without a
     branch and a residual_scale x' is x, and is only stored into x_out).
     post_norm / pre_norm: ND_NORM_NONE, _RMS or _LAYER, times post_weight /
-    pre_weight [width] (+ 1 with plus_one). gate, scale, shift: [width], or
+    pre_weight [width] (+ 1 with plus_one); pre_norm is _LAYER unless given,
+    where y is made. gate, scale, shift: [width], or
     [vecs, width] of one row stride: row r reads set min(r // rows_per_vec,
     vecs - 1). out_dtype None: x' only; torch.int8: one scale per row.
     Returns (x', y), (x', q, y_scale) for int8, or (x', None).
@@ -372,6 +373,8 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *, x_out:
         raise ValueError("residual_norm: out_scale goes with an int8 output")
     if out is not None:
         y_ptr, y_type = out.data_ptr(), _DT8[out_dtype]
+    if pre_norm is None:
+        pre_norm = _lib.ND_NORM_NONE if out is None else _lib.ND_NORM_LAYER
     a = _pack_residual_norm(rows, width, x_ptr, ldx, xo_ptr, ldo, b_ptr, ldb, b_type, post_norm, post_ptr, ptrs[0],
                             residual_scale, pre_norm, pre_ptr, ptrs[1], ptrs[2], vecs or 1, vec_stride, rows_per_vec,
                             1 if plus_one else 0, eps, y_ptr, ldy, y_type, q_ptr)

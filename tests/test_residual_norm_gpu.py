@@ -371,3 +371,14 @@ def test_an_exact_half_goes_to_even(cuda):
     _, q, scale = ops.residual_norm(x, pre_norm=NONE, out_dtype=I8)
     ops.sync()
     assert q[0].tolist() == [127, 0, 0, 2, -2, 2] and scale[0] == 3
+
+
+def test_only_x_without_naming_a_norm(cuda):
+    from naivediffusion_b200 import ops
+    x, b, v, _, _ = _inputs(40, 1280, F16, 1, 5)
+    keep = x.clone()
+    new, none = ops.residual_norm(x, b, x_out=torch.empty_like(x), gate=v[0, 0], out_dtype=None)
+    ops.sync()
+    xn, dx, _, _ = residual_norm64(x, b, gate=v[0, 0])
+    check(new, xn, dx)
+    assert none is None and torch.equal(x, keep)

@@ -153,3 +153,16 @@ def test_struct_layouts_match_the_header(tmp_path):
         assert C.sizeof(cls) == next(sizes), name
         for f in cls._fields_:
             assert getattr(cls, f[0]).offset == next(sizes), (name, f[0])
+
+
+def test_the_norm_defaults_to_layer_norm_where_y_is_made(monkeypatch):
+    """out_dtype None asks for x' only, and the call then names no norm."""
+    calls = []
+    monkeypatch.setattr(ops, "_launch", lambda what, device, fn, args: calls.append(_lib.ResidualNormArgs.from_buffer_copy(args)))
+    x, b = torch.zeros(4, 32), torch.zeros(4, 32)
+    for kw, want in (({}, _lib.ND_NORM_LAYER), (dict(out_dtype=None), _lib.ND_NORM_NONE), (dict(out_dtype=I8), _lib.ND_NORM_LAYER),
+                     (dict(out=torch.zeros(4, 32), out_dtype=None), _lib.ND_NORM_LAYER), (dict(pre_norm=1), _lib.ND_NORM_RMS),
+                     (dict(pre_norm=0), _lib.ND_NORM_NONE)):
+        ops.residual_norm(x, b, **kw)
+        assert calls[-1].pre_norm == want, kw
+    assert calls[1].y is None and calls[1].x_out == x.data_ptr()
