@@ -344,7 +344,7 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *, x_out:
         sets, wide, stride = _matrix(name, t if t.dim() != 1 else t[None], _FP32, device)
         if vecs == 0:
             vecs, vec_stride = sets, stride
-        if wide != width or sets != vecs or stride != vec_stride:
+        if wide != width or sets == 0 or sets != vecs or stride != vec_stride:
             raise ValueError(f"{name} must be [{width}] or [vecs, {width}] with the others' number of sets and row stride, "
                              f"got {tuple(t.shape)} with stride {stride}")
         ptrs[i] = t.data_ptr()

@@ -166,3 +166,10 @@ def test_the_norm_defaults_to_layer_norm_where_y_is_made(monkeypatch):
         ops.residual_norm(x, b, **kw)
         assert calls[-1].pre_norm == want, kw
     assert calls[1].y is None and calls[1].x_out == x.data_ptr()
+
+
+@pytest.mark.parametrize("name", ["gate", "scale", "shift"])
+def test_residual_norm_refuses_no_vector_sets(name):
+    x = torch.zeros(4, 32)
+    with pytest.raises(ValueError, match=f"residual_norm: {name}"):
+        ops.residual_norm(x, torch.zeros(4, 32), **{name: torch.zeros(0, 32)})
