@@ -401,7 +401,7 @@ def quantize_rows(x: torch.Tensor, *, out: torch.Tensor | None = None,
 
 
 def linear_w8a8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, w_scale: torch.Tensor,
-                bias: torch.Tensor | None = None, *, epilogue: int = _lib.ND_EPI_STORE, out_dtype=torch.bfloat16,
+                bias: torch.Tensor | None = None, *, epilogue: int = _lib.ND_EPI_STORE, out_dtype=None,
                 out: torch.Tensor | None = None, residual: torch.Tensor | None = None,
                 gate: torch.Tensor | None = None, group_split: int | None = None, shared_weights: bool = False,
                 addend: torch.Tensor | None = None) -> torch.Tensor:
@@ -413,7 +413,9 @@ def linear_w8a8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, w_
     scale_dtype=torch.float32)). rows >= group_split use the second group of
     weight rows, or with shared_weights only the second bias / gate. Residual
     epilogues update `residual` (fp32) in place and return it; STORE_F32 makes
-    one if none is given. SWIGLU / GEGLU: weight [2F, in], output [rows, F].
+    one if none is given; the others write `out`, or a new matrix of out_dtype
+    (bfloat16 unless given). SWIGLU / GEGLU: weight [2F, in], output [rows, F].
+    gate goes with RESIDUAL_GATE, addend with ADD_STORE.
     """
     device = x.device
     rows, k, ldx = _matrix("linear_w8a8: x", x, _INT8, device, 16)
@@ -429,8 +431,14 @@ def linear_w8a8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, w_
     sw_ptr = _vector("linear_w8a8: w_scale", w_scale, w_rows, device)
     bias_ptr = _vector("linear_w8a8: bias", bias, (2 if split else 1) * each, device)
     gate_ptr = _vector("linear_w8a8: gate", gate, (2 if split else 1) * n, device)
+    if (gate is not None) != (epilogue == _lib.ND_EPI_RESIDUAL_GATE):
+        raise ValueError("linear_w8a8: gate goes with RESIDUAL_GATE, and RESIDUAL_GATE with a gate")
+    if (addend is not None) != (epilogue == _lib.ND_EPI_ADD_STORE):
+        raise ValueError("linear_w8a8: addend goes with ADD_STORE, and ADD_STORE with an addend")
     y_ptr = ldy = r_ptr = ldr = a_ptr = lda = 0
     if epilogue in _RESIDUAL_EPI:
+        if out is not None or (out_dtype is not None and out_dtype is not _F32):
+            raise ValueError("linear_w8a8: this epilogue writes residual in float32, and takes no out nor another out_dtype")
         if residual is not None:
             ldr = _output("linear_w8a8: residual", residual, rows, n, _FP32, device, 4)
         elif epilogue == _lib.ND_EPI_STORE_F32:
@@ -439,13 +447,19 @@ def linear_w8a8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, w_
             raise ValueError("linear_w8a8: this epilogue adds to residual, and none is given")
         result, r_ptr, out_dtype = residual, residual.data_ptr(), torch.bfloat16
     else:
+        if residual is not None:
+            raise ValueError("linear_w8a8: this epilogue writes out, and takes no residual")
         if out is not None:
             ldy = _output("linear_w8a8: out", out, rows, n, _HALVES, device, 8)
+            if out_dtype is not None and out_dtype != out.dtype:
+                raise ValueError(f"linear_w8a8: out_dtype is {out_dtype}, out is {out.dtype}")
             out_dtype = out.dtype
-        elif out_dtype in _HALVES:
-            out, ldy = _padded(rows, n, 8, device, out_dtype)
         else:
-            raise ValueError(f"linear_w8a8: out_dtype must be float16 or bfloat16 (STORE_F32 for fp32), got {out_dtype}")
+            if out_dtype is None:
+                out_dtype = torch.bfloat16
+            if out_dtype not in _HALVES:
+                raise ValueError(f"linear_w8a8: out_dtype must be float16 or bfloat16 (STORE_F32 for fp32), got {out_dtype}")
+            out, ldy = _padded(rows, n, 8, device, out_dtype)
         result, y_ptr = out, out.data_ptr()
     if addend is not None:
         lda = _output("linear_w8a8: addend", addend, rows, n, (out_dtype,), device)

@@ -173,3 +173,27 @@ def test_residual_norm_refuses_no_vector_sets(name):
     x = torch.zeros(4, 32)
     with pytest.raises(ValueError, match=f"residual_norm: {name}"):
         ops.residual_norm(x, torch.zeros(4, 32), **{name: torch.zeros(0, 32)})
+
+
+def test_linear_w8a8_refuses_what_it_would_not_use(monkeypatch):
+    x, sx, w, sw = torch.zeros(8, 64, dtype=I8), torch.zeros(8), torch.zeros(32, 64, dtype=I8), torch.zeros(32)
+    y, r, add, gate = torch.zeros(8, 32).bfloat16(), torch.zeros(8, 32), torch.zeros(8, 32).bfloat16(), torch.zeros(32)
+    E = _lib
+    for match, kw in (("out", dict(epilogue=E.ND_EPI_STORE_F32, out=y)), ("out", dict(epilogue=E.ND_EPI_RESIDUAL_ADD, residual=r, out=y)),
+                      ("out_dtype", dict(epilogue=E.ND_EPI_STORE_F32, out_dtype=torch.float16)),
+                      ("out_dtype", dict(epilogue=E.ND_EPI_RESIDUAL_ADD, residual=r, out_dtype=torch.bfloat16)),
+                      ("out_dtype", dict(out=y, out_dtype=torch.float16)),
+                      ("residual", dict(residual=r)), ("residual", dict(epilogue=E.ND_EPI_SILU, residual=r)),
+                      ("addend", dict(addend=add)), ("addend", dict(epilogue=E.ND_EPI_STORE_F32, addend=add)),
+                      ("addend", dict(epilogue=E.ND_EPI_ADD_STORE)),
+                      ("gate", dict(gate=gate)), ("gate", dict(epilogue=E.ND_EPI_RESIDUAL_ADD, residual=r, gate=gate)),
+                      ("gate", dict(epilogue=E.ND_EPI_RESIDUAL_GATE, residual=r))):
+        with pytest.raises(ValueError, match=f"linear_w8a8: .*{match}"):
+            ops.linear_w8a8(x, sx, w, sw, **kw)
+    monkeypatch.setattr(ops, "_launch", lambda *args: None)
+    for kw, dtype in (({}, torch.bfloat16), (dict(out_dtype=torch.float16), torch.float16), (dict(out=y), torch.bfloat16),
+                      (dict(out=y, out_dtype=torch.bfloat16), torch.bfloat16), (dict(epilogue=E.ND_EPI_STORE_F32), torch.float32),
+                      (dict(epilogue=E.ND_EPI_STORE_F32, out_dtype=torch.float32, residual=r), torch.float32),
+                      (dict(epilogue=E.ND_EPI_ADD_STORE, addend=add), torch.bfloat16),
+                      (dict(epilogue=E.ND_EPI_RESIDUAL_GATE, residual=r, gate=gate), torch.float32)):
+        assert ops.linear_w8a8(x, sx, w, sw, **kw).dtype == dtype
