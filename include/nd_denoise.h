@@ -499,8 +499,10 @@ ND_API int nd_op_residual_norm(const nd_residual_norm_args* args, void* stream);
  *   scale[r] = max |x[r]| / 127,  q[r, c] = rint(x[r, c] * 127 / max |x[r]|)
  * with the quotient rounded as if exact, half to even. A row of zeros has
  * scale 0; a row that holds an infinity or a NaN has scale NaN and q 0.
- * Columns of q at and past cols are not written. The weights' counterpart is
- * nd_op_quantize (quant_group 0: one scale per output channel). */
+ * Columns of q at and past cols are not written. It makes weights too, one
+ * scale per output channel, with any row stride; nd_op_quantize (quant_group
+ * 0), which multiplies by 1 / scale instead, writes rows cols bytes apart,
+ * which nd_op_linear_w8a8 reads where cols is a multiple of 16. */
 ND_API int nd_op_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int8_t* q,
                                int64_t ldq, float* scale, void* stream);
 
@@ -508,7 +510,8 @@ ND_API int nd_op_quantize_rows(const void* x, int dtype, int64_t rows, int64_t c
  * y[r, c] = epilogue(x_scale[r] * w_scale[c] * sum_k x[r, k] * weight[c, k] + bias[c])
  * with int8 x (one scale per row: nd_op_quantize_rows, or nd_op_residual_norm
  * with an int8 y) and int8 weight (one scale per output channel:
- * nd_op_quantize with quant_group 0 and fp32 scales). The sum is exact in 32-bit
+ * nd_op_quantize with quant_group 0 and fp32 scales where in_features is a
+ * multiple of 16, nd_op_quantize_rows for any). The sum is exact in 32-bit
  * integers (in_features < 131072). nd_op_linear's weight-only int8 widens the
  * weights and multiplies in 16 bits; this is the 8-bit product itself.
  * Row groups (group_split, shared_weights), the epilogues and their operands

@@ -386,7 +386,7 @@ def quantize_rows(x: torch.Tensor, *, out: torch.Tensor | None = None,
                   scale: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Rows (tokens) as int8 with one scale each: scale = max |x| / 127 over the row, q = rint(x * 127 / max |x|),
     the quotient rounded as if exact. Returns (q [rows, cols], scale [rows]); q's rows are a multiple of 16 bytes
-    apart, as linear_w8a8 reads them. A row with an infinity or a NaN gets scale NaN and q 0."""
+    apart, as linear_w8a8 reads them: its x, or a weight with any number of inputs. A row with an infinity or a NaN gets scale NaN and q 0."""
     device = x.device
     rows, cols, ldx = _matrix("quantize_rows: x", x, _FLOATS, device)
     if out is None:
@@ -409,8 +409,9 @@ def linear_w8a8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, w_
 
     x [rows, in] and x_scale [rows] as quantize_rows or residual_norm write
     them; weight [groups * out, in] int8 (row stride a multiple of 16) with
-    w_scale, one per weight row (quantize(w, quant_group=0,
-    scale_dtype=torch.float32)). rows >= group_split use the second group of
+    w_scale, one per weight row: quantize(w, quant_group=0,
+    scale_dtype=torch.float32) where in is a multiple of 16, quantize_rows(w)
+    for any. rows >= group_split use the second group of
     weight rows, or with shared_weights only the second bias / gate. Residual
     epilogues update `residual` (fp32) in place and return it; STORE_F32 makes
     one if none is given; the others write `out`, or a new matrix of out_dtype

@@ -388,3 +388,18 @@ def test_more_gated_outputs_than_warps_count_in_32_bits(cuda):
     want[:50], want[n - 100:] = 4 * one, two
     # two fp32 roundings of the factors, ex2 and rcp a few ulp each, and the store's half step
     assert (out[0].float() - want).abs().le(want * (2.0 ** -8 + 16 * U)).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 96, 77), (20, 130, 1155), (200, 64, 333), (1100, 512, 71)])
+def test_weights_of_any_width(cuda, m, n, k):
+    """quantize_rows makes weights too, of any in_features: rows a multiple of 16 bytes apart, a scale per channel."""
+    from naivediffusion_b200 import ops
+    g = _gen(m + k)
+    wf = torch.randn(n, k, generator=g, device="cuda") / math.sqrt(k)
+    x, sx = ops.quantize_rows(torch.randn(m, k, generator=g, device="cuda"))
+    w, sw = ops.quantize_rows(wf)
+    y = ops.linear_w8a8(x, sx, w, sw)
+    ops.sync()
+    check(w.double() * sw.double()[:, None], wf.double(), sw.double()[:, None] * 0.5 + 2 * U * wf.abs())
+    v, dv = linear64(x, sx, w, sw)
+    check(y, v, dv + half_step(v.abs() + dv, BF16))
