@@ -550,19 +550,14 @@ int dequantize(const int8_t* q, const void* scales, int scale_dtype, int64_t qua
   const int64_t group = quant_group > 0 ? quant_group : cols;
   if (cols % group) return fail(ND_ERR_INVALID, "dequantize: quant_group must divide cols");
   const bool aligned = reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
-  const int64_t runs = (rows * cols + 16 * 256 - 1) / (16 * 256);
-  const int f16 = scale_dtype == ND_F16, g = static_cast<int>(group), w = static_cast<int>(cols);
+  const bool by16 = aligned && group >= 16;
+  const int64_t total = rows * cols, per_block = 256 * (by16 ? 16 : kDequantValues);
+  const int64_t blocks = (total + per_block - 1) / per_block;
+  if (blocks > INT_MAX) return fail(ND_ERR_INVALID, "dequantize: shape too large");
+  const int f16 = scale_dtype == ND_F16, g = static_cast<int>(group), to_f16 = out_dtype == ND_F16;
   uint16_t* o = static_cast<uint16_t*>(out);
-  if (aligned && group >= 16 && runs <= INT_MAX) {
-    dequant_runs_kernel<<<static_cast<unsigned>(runs), 256, 0, stream>>>(q, scales, f16, rows * cols, g, o, out_dtype == ND_F16);
-  } else {
-    const int64_t per_row = (cols + 127) / 128;  // blocks to cover a row at once
-    const int64_t most = sm_count() * 16LL;
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(rows, most)),
-                    static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(per_row, most / std::min<int64_t>(rows, most)))));
-    dequant_w8_kernel<<<grid, 128, 0, stream>>>(q, scales, f16, g, static_cast<int>(cols / group), rows, w, o,
-                                                out_dtype == ND_F16);
-  }
+  auto kernel = by16 ? dequant_runs_kernel : group < 256 ? dequant_values_kernel<false> : dequant_values_kernel<true>;
+  kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(q, scales, f16, total, g, o, to_f16);
   ND_CUDA(cudaGetLastError());
   return ND_OK;
 }

@@ -382,3 +382,22 @@ def test_only_x_without_naming_a_norm(cuda):
     xn, dx, _, _ = residual_norm64(x, b, gate=v[0, 0])
     check(new, xn, dx)
     assert none is None and torch.equal(x, keep)
+
+
+@pytest.mark.parametrize("rows,cols,group,start", [(5000, 1, 1, 0), (7001, 3, 3, 1), (3000, 8, 4, 0), (1001, 15, 15, 5), (513, 33, 33, 1),
+                                                   (400, 129, 43, 3), (1000, 1155, 1155, 3), (301, 768, 256, 3), (77, 510, 255, 1),
+                                                   (9, 771, 257, 7), (3, 40000, 8, 0), (2, 5000, 2500, 1)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_values_of_any_rows_and_groups(cuda, rows, cols, group, start, dtype):
+    """Narrow rows, short groups, and long ones off a 16-byte address, bit for bit; nothing past the last value."""
+    from naivediffusion_b200 import _lib, ops
+    g = _gen(rows + cols)
+    q = torch.randint(-127, 128, (rows * cols + start,), generator=g, device="cuda", dtype=torch.int32).to(I8)[start:].view(rows, cols)
+    scale = _randn(g, rows, cols // group).abs()
+    want = (q.float().view(rows, -1, group) * scale[:, :, None]).to(dtype).flatten()
+    out = torch.full((rows * cols + 40,), 7, device="cuda", dtype=dtype)
+    _lib.check(_lib.lib().nd_op_dequantize(q.data_ptr(), scale.data_ptr(), _lib.ND_F32, group, rows, cols, out.data_ptr(),
+                                           ops._DT[dtype], torch.cuda.current_stream().cuda_stream))
+    ops.sync()
+    assert torch.equal(out[:rows * cols], want) and out[rows * cols:].eq(7).all()
+    assert torch.equal(ops.dequantize(q, scale, group, dtype).flatten(), want)
