@@ -89,3 +89,19 @@ def test_what_lies_beside_two_groups_stays(cuda, m, split, n, weights):
         ops.sync()
         assert torch.equal(store[:, :n], (sums + (5 if epi == ADD else 0)).to(store.dtype)), epi
         assert store[:, n:].eq(5).all(), epi
+
+
+@pytest.mark.parametrize("m,n", [(50, 101), (300, 202), (1100, 1023)])
+def test_what_lies_beside_fp32_compute_stays(cuda, m, n):
+    """The residual epilogues on bf16 pairs (hi | lo), whose fp32 output may have any width."""
+    from naivediffusion_b200 import ops
+    k, g = 64, torch.Generator(device="cuda").manual_seed(m)
+    x, w = _whole(g, -3, 3, m, k), _whole(g, -2, 2, n, k)
+    sums = x @ w.t()
+    wide = -(-n // 4) * 4 + 16
+    for epi in (STORE_F32, ADD):
+        store = torch.full((m + 2, wide), 5.0, device="cuda")
+        ops.linear(ops.to_pairs(x), ops.to_pairs(w), epilogue=epi, pairs=True, residual=store[:, :n])
+        ops.sync()
+        assert torch.equal(store[:m, :n], sums + (5 if epi == ADD else 0)), epi
+        assert store[m:].eq(5).all() and store[:m, n:].eq(5).all(), epi
