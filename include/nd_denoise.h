@@ -308,9 +308,10 @@ typedef struct nd_linear_args {
   const void* weight;   /* [groups * out_features, in_features], row-major */
   const float* bias;    /* [groups * out_features] or NULL */
   int64_t group_split;  /* first row of group 1; >= rows for one group */
-  void* y;              /* [rows, ldy] (ND_EPI_STORE, GELU*, SILU, QK_NORM_ROPE) */
+  void* y;              /* [rows, ldy] (ND_EPI_STORE, GELU*, SILU, QK_NORM_ROPE); columns past
+                           out_features, of any width, stay as they are */
   int64_t ldy;
-  float* residual;      /* [rows, ldr] fp32 (RESIDUAL_*, STORE_F32) */
+  float* residual;      /* [rows, ldr] fp32 (RESIDUAL_*, STORE_F32), likewise */
   int64_t ldr;
   const float* gate;    /* [groups][gate_stride] (RESIDUAL_GATE) */
   int64_t gate_stride;  /* 0: out_features */
@@ -516,7 +517,8 @@ ND_API int nd_op_quantize_rows(const void* x, int dtype, int64_t rows, int64_t c
  * weights and multiplies in 16 bits; this is the 8-bit product itself.
  * Row groups (group_split, shared_weights), the epilogues and their operands
  * are nd_linear_args'; QK_NORM_ROPE is not offered (nd_op_head_norm_rope runs
- * after a STORE). Repeated calls give the same bits. There is no workspace:
+ * after a STORE). Repeated calls give the same bits, and a row's do not depend
+ * on group_split beyond the group that it is in. There is no workspace:
  * calls on different streams, and captured ones, share nothing. The first call
  * on a device (this one's or nd_op_residual_norm's) allocates the library's
  * status word: make it before a stream capture. */

@@ -11,10 +11,13 @@
 // At twice the 16-bit rate a tile's MMAs last half as long per k, so the
 // epilogue has eight warps per CTA (two per TMEM lane quarter, each half of
 // the tile's columns) instead of four; sixteen warps of sixteen columns
-// measured even (4096 x 640 x 5120 GEGLU 34-37 us both).
+// measured even (4096 x 640 x 5120 GEGLU 34-40 us both).
 //
-// 4352 x 4096 x 24576 SwiGLU: 271-278 us, 3.15-3.23 POP/s, the tensor pipe 95 %
-// active (ncu); 4352 x 12288 x 4096: 139 us, 3.15 POP/s (3.68 rounds of pairs).
+// 4352 x 4096 x 24576 SwiGLU: 266-278 us in bursts, 3.15-3.29 POP/s, the tensor
+// pipe 95 % active (ncu), 318 us back to back at 1.28 GHz; 4352 x 12288 x 4096: 139
+// us, 3.15 POP/s (3.68 rounds of pairs), and 168 at 1.35 GHz; its RESIDUAL
+// epilogues 147 and 176, ADD_STORE, whose lanes read the addend two bytes at a
+// time, 211 and 241.
 // Below about K = 2048 the epilogue bounds it (4096 x 640 x 5120 GEGLU: 1.5
 // POP/s, tensor pipe 37 %).
 #pragma once

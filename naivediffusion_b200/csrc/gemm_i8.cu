@@ -22,12 +22,16 @@ constexpr int kFewRows = 32;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// Launch a kernel whose clusters of S CTAs share a tile's k blocks. A k block
-// takes block_us on one SM (both kernels run at the rate an SM takes bytes
-// from L2, about 106 GB/s), and a split costs fixed_us + S * each_us for the
-// cluster barriers and the sums' way through the cluster's shared memory
-// (measured per kernel). S is the cheapest count whose clusters all run at
-// once (`most`, looked up once per kernel and device).
+// Launch a kernel whose clusters of S CTAs share a tile's k blocks. The rule
+// counts block_us for a k block on one SM, and fixed_us + S * each_us for a
+// split: the cluster barriers and the sums' way through the cluster's shared
+// memory: estimates, one set per kernel. S is the cheapest count whose clusters
+// all run at once (`most`, looked up once per kernel and device).
+//
+// What a k block takes without a split, from the times' slope over K: the
+// 128 x 128 kernel's 32 KB 0.19-0.23 us with 144 tiles at once (140-170 GB/s per
+// SM); the few-rows kernel's 18 KB 0.155 us with 96 tiles and the weights in L2
+// (119 GB/s per SM), 0.23-0.28 us once they come from HBM.
 struct SplitCost {
   float block_us, fixed_us, each_us;
 };
@@ -143,10 +147,11 @@ int launch_i8_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorM
   return ND_OK;
 }
 
-// Pair or one-SM kernel. A k block of either takes an SM its 32 KB at the rate
-// it takes bytes from L2, 0.30 us, for a 128 x 256 share of a pair tile or
-// for a 128 x 128 tile (whose missing rows cost nothing); what counts is the
-// number of rounds. Pair / one-SM, us: 256 x 4096 x 12288 18.3 / 23.8,
+// Pair or one-SM kernel. Either loads 32 KB per k block and SM, the pair kernel
+// for a 128 x 256 share of its tile (0.32-0.35 us with one round of pairs), the
+// one-SM kernel for 128 x 128 (0.19-0.23 us; missing rows cost nothing); the rule
+// compares the rounds that both need, and its crossings were measured. Pair /
+// one-SM, us: 256 x 4096 x 12288 18.3 / 23.8,
 // 512 x 4096 x 4096 16.1 / 12.2, 1024 x 4096 x 4096 17.2 / 22.7,
 // 1024 x 640 x 2048 7.9 / 6.4.
 bool pair_is_faster(int64_t rows, int64_t n) {

@@ -65,7 +65,9 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
 // A warp's columns of the per-column vectors, staged in its own shared memory
 // while the tile's MMAs run. With that, the paired fp32 arithmetic and the ex2 /
 // rcp activations below the pair kernel's 8192 x 2048 x 8192 GELU went from
-// 132 to 100 us (25 to 13 instructions per output):
+// 132 to 100 us on one box (25 to 13 instructions per output). It depends on the
+// clock: 100-115 us in bursts, 127-134 us back to back at 1.49 GHz (erf 111 and
+// 133, SILU 106 and 127, STORE 91 and 110):
 //   words [0, 128)    w_scale     (gated: the first factor's 64, then the second's)
 //   words [128, 256)  bias        (likewise)
 //   words [256, 384)  gate

@@ -6,7 +6,9 @@
 // gated epilogues): lane l reads 16-byte groups l, l + 32, .. of both rows,
 // kGroups of each in flight, against the same groups of x, which stay in L1.
 // One warp per pair of rows and about one wave of blocks, so every load of the
-// weights is in flight early: 1 x 4096 x 12288 9.5 us (5.3 TB/s). Two rows of x
+// weights is in flight early: 1 x 4096 x 12288 9.5 us (5.3 TB/s) over three
+// layers' weights in turn (150 MB, which L2 partly holds), 10.8 us (4.7 TB/s) over
+// twelve layers' (600 MB). Two rows of x
 // take two groups and 48 warps per SM (10.2 us against 12.4 with four groups);
 // one, three and four rows lose by that (4 x 4096 x 12288 12.9 against 18.4).
 #pragma once
