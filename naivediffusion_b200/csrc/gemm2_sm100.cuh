@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(192, 1)
               tmem_ld_wait();
               GemmArgs plain = args;
               plain.epi = kEpiStore;
-              epilogue_chunk(plain, &tmC, group, row0, col0 + c * 32, r, buf0, sb, lane);
+              epilogue_chunk<false>(plain, &tmC, group, row0, col0 + c * 32, r, buf0, sb, lane);
             }
           }
         }
@@ -364,7 +364,7 @@ __global__ void __launch_bounds__(192, 1)
           uint32_t r[32];
           tmem_ld32(tbase + c * 32, r);
           tmem_ld_wait();
-          epilogue_chunk(args, &tmC, group, row0, col, r, buf0, sb, lane);
+          epilogue_chunk<!CONV>(args, &tmC, group, row0, col, r, buf0, sb, lane);
         }
       }
       tc_fence_before();
