@@ -337,7 +337,7 @@ typedef struct nd_linear_args {
    * (0 = row), for batch items stacked by rows. */
   int64_t norm_span;
   int64_t rope_period;
-  const void* addend;   /* ADD_STORE: [rows, ld_add], dtype like y */
+  const void* addend;   /* ADD_STORE: [rows, ld_add], dtype like y, 16-byte aligned */
   int64_t ld_add;
   int shared_weights;   /* 1: one weight matrix for both row groups (see above) */
 } nd_linear_args;
@@ -362,7 +362,7 @@ typedef struct nd_conv_args {
   int64_t bias_stride;  /* per_batch_bias: floats between batch items' bias vectors (0: out_channels) */
   void* y;              /* [batch, H_out, W_out, out_channels] */
   float* y_f32;         /* STORE_F32 output */
-  const void* addend;   /* ADD_STORE: like y */
+  const void* addend;   /* ADD_STORE: like y, 16-byte aligned */
 } nd_conv_args;
 
 ND_API int nd_op_conv2d(const nd_conv_args* args, void* stream);

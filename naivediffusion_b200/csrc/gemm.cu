@@ -333,8 +333,9 @@ int linear(const nd_linear_args& a, cudaStream_t stream) {
   if (epi < 0 || epi > ND_EPI_GEGLU) return fail(ND_ERR_INVALID, "linear: unknown epilogue");
   const bool swiglu = epi == ND_EPI_SWIGLU || epi == ND_EPI_GEGLU;
   if (swiglu && a.out_features % 128) return fail(ND_ERR_INVALID, "linear: SWIGLU / GEGLU need out_features % 128 == 0");
-  if (epi == ND_EPI_ADD_STORE && (!a.addend || a.ld_add < a.out_features || a.ld_add % 8 != 0))
-    return fail(ND_ERR_INVALID, "linear: ADD_STORE needs addend with ld_add >= out_features, ld_add % 8 == 0");
+  if (epi == ND_EPI_ADD_STORE &&
+      (!a.addend || a.ld_add < a.out_features || a.ld_add % 8 != 0 || (reinterpret_cast<uintptr_t>(a.addend) & 15u)))
+    return fail(ND_ERR_INVALID, "linear: ADD_STORE needs a 16-byte aligned addend with ld_add >= out_features, ld_add % 8 == 0");
   if (resid && (!a.residual || a.ldr < a.out_features || a.ldr % 4 != 0))
     return fail(ND_ERR_INVALID, "linear: residual epilogue needs residual with ldr >= out_features, ldr % 4 == 0");
   if (!resid && (!a.y || a.ldy < a.out_features || a.ldy % 8 != 0))
@@ -468,7 +469,8 @@ int conv2d(const nd_conv_args& c, cudaStream_t stream) {
     return fail(ND_ERR_INVALID, "conv2d: epilogue must be STORE, ADD_STORE, STORE_F32 or SILU");
   if (!c.x || !c.weight) return fail(ND_ERR_INVALID, "conv2d: null operand");
   if (epi == ND_EPI_STORE_F32 ? !c.y_f32 : !c.y) return fail(ND_ERR_INVALID, "conv2d: null output");
-  if (epi == ND_EPI_ADD_STORE && !c.addend) return fail(ND_ERR_INVALID, "conv2d: ADD_STORE needs addend");
+  if (epi == ND_EPI_ADD_STORE && (!c.addend || (reinterpret_cast<uintptr_t>(c.addend) & 15u)))
+    return fail(ND_ERR_INVALID, "conv2d: ADD_STORE needs a 16-byte aligned addend");
   if (epi != ND_EPI_STORE_F32 && c.out_channels % 8) return fail(ND_ERR_INVALID, "conv2d: out_channels % 8 for a 16-bit output");
   if (c.out_channels % 4) return fail(ND_ERR_INVALID, "conv2d: out_channels must be a multiple of 4");
   const int64_t M = static_cast<int64_t>(c.batch) * ho * wo;

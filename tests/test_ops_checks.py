@@ -49,3 +49,17 @@ def test_sampler_step_rejects_mismatched_buffers():
         ops.sampler_step(0, 0, torch.zeros(32), s, last=torch.zeros(8), sigma=1.0, sigma_next=0.5)
     with pytest.raises(ValueError, match="next_input"):
         ops.sampler_step(0, 0, s, s, next_input=torch.zeros(16, dtype=torch.float16), sigma=1.0, sigma_next=0.5)
+
+
+def test_an_addend_off_16_bytes_is_refused():
+    """linear and conv2d read it as 16-byte vectors."""
+    import ctypes as C
+    P = 1 << 20  # a 16-byte aligned address that is never read: every call here is refused
+    L = _lib.lib()
+    lin = _lib.LinearArgs(dtype=_lib.ND_BF16, epilogue=_lib.ND_EPI_ADD_STORE, rows=8, in_features=64, out_features=64, x=P, ldx=64,
+                          weight=P, group_split=8, y=P, ldy=64, addend=P + 8, ld_add=64)
+    conv = _lib.ConvArgs(dtype=_lib.ND_BF16, epilogue=_lib.ND_EPI_ADD_STORE, batch=1, height=16, width=16, in_channels=64,
+                         out_channels=64, stride=1, x=P, weight=P, y=P, addend=P + 2)
+    for fn, args in ((L.nd_op_linear, lin), (L.nd_op_conv2d, conv)):
+        assert fn(C.byref(args), None) == _lib.ND_ERR_INVALID
+        assert "16-byte aligned addend" in L.nd_last_error().decode()
